@@ -281,7 +281,7 @@ def _handles(st):
         d = _lib.NhVerifyDrafts(
             target=p(st["target"]), target_stride=c["n_vocab"], draft=p(st["draft"]), draft_stride=c["n_vocab"],
             draft_ids=p(st["ids"]), draft_off=p(st["off"]), u_accept=p(st["u_accept"]), u_pick=p(st["u_pick"]),
-            n_seq=c["n_seq"], max_draft=st["most"], n_vocab=c["n_vocab"], n_accept=p(st["n_accept"]),
+            n_seq=c["n_seq"], n_drafts=st["ids"].numel(), max_draft=st["most"], n_vocab=c["n_vocab"], n_accept=p(st["n_accept"]),
             out_ids=p(st["out_ids"]), err=None)
         return lib, ctypes.byref(d), d
     kv = st["kv"]

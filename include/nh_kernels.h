@@ -34,6 +34,7 @@ extern "C" {
 #define NH_TYPE_F32 0
 #define NH_TYPE_Q4_K 12
 #define NH_TYPE_Q6_K 14
+#define NH_TYPE_BF16 30 /* nh_paged_read's outputs only */
 
 #define NH_OK 0
 #define NH_E_ARG (-1)         /* bad argument (null pointer, size, unsupported shape) */
@@ -418,6 +419,128 @@ int nh_prefill_qk_seqs(const float* q, const float* k, const float* v, const flo
 int nh_prefill_attention_seqs(const float* qr, int n_seq, int n_tok, int pos0, int n_head, int n_head_kv,
                               int head_dim, float kq_scale, const float* k_cache, const float* v_cache, int max_seq,
                               float* out, void* stream);
+
+/* ---- paged 8-bit K/V cache: sequences of unequal lengths, any number of rows
+ * each per call (one decode position, drafted positions, a prompt chunk), over
+ * a cache a quarter the size of the f32 one (no reference counterpart; the
+ * paged form of KvCache, kv_cache.h:14-35, under BuildAttentionCached,
+ * attention.cc:65-135).  One step of a layer is
+ *   nh_paged_append -> nh_paged_attention
+ * with the same NhPagedKv and NhPagedRows.
+ *
+ * Storage.  A page holds page_size consecutive positions of one sequence, per
+ * KV head as [page_size][head_dim] unsigned 8-bit codes, and one f32 scale per
+ * KV head for the keys and one for the values.  Code u stands for
+ * (u - 127.5) * scale.  A scale is a power of two: with 2^E <= m < 2^(E+1) for
+ * the largest magnitude m of the page's head so far, scale = 2^(E-6) (at least
+ * 2^-106) and u = floor(x / scale) + 128, an error of at most scale / 2.
+ * A page that fills over several calls keeps its scale until a row needs a
+ * larger one; the codes it holds are then moved to that scale by an arithmetic
+ * shift.  Since floor(floor(x / s) / 2) = floor(x / 2s), a page's codes depend
+ * on its rows and its scale alone, not on how the rows were split over calls.
+ * A page whose first position is written again starts afresh; lowering pos0
+ * inside a page (drafts that were refused) keeps the page's scale. */
+typedef struct NhPagedKv {
+  uint8_t* k_codes;   /* [n_pages][n_head_kv][page_size][head_dim], 16-byte aligned */
+  uint8_t* v_codes;
+  float* k_scales;    /* [n_pages][n_head_kv] */
+  float* v_scales;
+  int32_t n_pages;
+  int32_t page_size;  /* 16, 32, 64 or 128 */
+  int32_t n_head_kv;
+  int32_t head_dim;   /* 32, 64, 96 or 128 */
+} NhPagedKv;
+
+/* The rows of one call: sequence s has rows row_off[s] .. row_off[s+1]-1 (none
+ * is fine), at positions pos0[s], pos0[s]+1, ...; its position p lies in page
+ * page_table[s*max_blocks + p / page_size].  The arrays are device memory and
+ * may change between replays of a captured call; n_rows (rows of the row
+ * buffers) and max_rows (most rows of one sequence) bound them.  A sequence
+ * outside those bounds or past max_blocks pages, and a page outside
+ * [0, n_pages), are not touched and record NH_E_ARG in *err (err may be null):
+ * such a sequence's rows are left as they were, such a page's positions are
+ * neither written nor seen.  Rows at and after row_off[n_seq] are left as they
+ * were.  A page that is written belongs to one sequence of the call; pages
+ * that are only read may be shared. */
+typedef struct NhPagedRows {
+  int32_t n_seq;      /* 1 .. 65535 */
+  int32_t max_rows;
+  int32_t n_rows;
+  int32_t max_blocks;
+  const int32_t* row_off;     /* [n_seq + 1], row_off[0] = 0 or more, not decreasing */
+  const int32_t* pos0;        /* [n_seq] */
+  const int32_t* page_table;  /* [n_seq][max_blocks] */
+  int32_t* err;
+} NhPagedRows;
+
+/* nh_prefill_qk for a paged cache: QK-norm over the full q and k width (with
+ * q_norm and k_norm both null: none), NEOX RoPE at each row's position, the
+ * rotated q into qr [n_rows][n_head*head_dim], and the rotated K and raw V rows
+ * coded into the cache.  Row r of q, k and v starts r * its stride floats in;
+ * rope_cs is nh_rope_table's table of rope_len positions (a sequence past it
+ * counts as out of bounds).  q and qr may both be null.  A K or V value that
+ * is not finite is coded as the nearest end of the range (a NaN as its middle),
+ * sets no scale, and records NH_E_ARG in *err.  Pointers are 16-byte aligned, strides
+ * a multiple of 4. */
+int nh_paged_append(const NhPagedKv* kv, const NhPagedRows* rows, const float* q, int64_t q_stride, const float* k,
+                    int64_t k_stride, const float* v, int64_t v_stride, const float* q_norm, const float* k_norm,
+                    float eps, int n_head, const float* rope_cs, int rope_len, float* qr, void* stream);
+
+/* Attention of each row over its sequence's cached positions, its own among
+ * them (append first): out[r] = sum_t softmax_t(kq_scale * qr[r].k_t) v_t over
+ * the positions t <= p of a row at position p with, when window > 0,
+ * t > p - window or t < n_sink (the window's positions and the first n_sink,
+ * which stay visible).  qr and out are [n_rows][n_head*head_dim], 16-byte
+ * aligned; any n_head that n_head_kv divides.  No scratch: a sequence with few
+ * rows is split over the CTAs of a cluster, joined in a fixed order, so equal
+ * calls give equal bits.  A row that sees no position gives zeros. */
+int nh_paged_attention(const NhPagedKv* kv, const NhPagedRows* rows, const float* qr, int n_head, float kq_scale,
+                       int window, int n_sink, float* out, void* stream);
+
+/* The values that the cache holds at the rows' positions, k_out and v_out
+ * [n_rows][n_head_kv*head_dim] (either may be null), as NH_TYPE_F32 or
+ * NH_TYPE_BF16 (both exact); to hand a sequence to another cache, or to check
+ * one.  Positions of a page outside [0, n_pages) read as zeros. */
+int nh_paged_read(const NhPagedKv* kv, const NhPagedRows* rows, int32_t out_type, void* k_out, void* v_out,
+                  void* stream);
+
+/* Checks each sequence's drafted tokens against the target's probabilities
+ * (the stochastic form of nh_batch_argmax for several positions at once; no
+ * reference counterpart).  Sequence s drafted ids draft_ids[o .. o+n-1], with o
+ * = draft_off[s] and n = draft_off[s+1] - o; target row o + s + i holds the
+ * target's probabilities at the position of draft i, row o + s + n those after
+ * the last.  Draft i is accepted while u_accept[o+i] * draft[o+i][id] <
+ * target[o+s+i][id].  The first refused draft is replaced by a token drawn from
+ * max(target - draft, 0) of its rows (from target, where that is zero
+ * everywhere); after n accepted ones the next token is drawn from the last
+ * target row.  The draw is the lowest id whose running sum exceeds
+ * u_pick[s] * the sum.  draft null: the drafts are certain (probability 1 at
+ * the drafted id, 0 elsewhere).  Products and sums are in 64 bits; an entry
+ * that is not above 0 (a NaN too) has no mass.  Rows need not sum to 1.
+ *   n_accept [n_seq]; out_ids [n_seq][max_draft+1]: the accepted ids, then the
+ *   drawn one; what follows is left as it was.
+ * A draft id outside [0, n_vocab) is refused; a row without mass draws id -1;
+ * both record NH_E_ARG in *err (may be null).  So does a sequence with n < 0 or
+ * n > max_draft or an offset outside [0, n_drafts]; nothing is written for it.
+ * Every row is at most 2^31-1 ids long. */
+typedef struct NhVerifyDrafts {
+  const float* target;    /* [n_drafts + n_seq] rows */
+  int64_t target_stride;  /* floats between rows */
+  const float* draft;     /* [n_drafts] rows, or null */
+  int64_t draft_stride;
+  const int32_t* draft_ids;  /* [n_drafts] */
+  const int32_t* draft_off;  /* [n_seq + 1] */
+  const float* u_accept;     /* [n_drafts], in [0, 1) */
+  const float* u_pick;       /* [n_seq], in [0, 1) */
+  int32_t n_seq;
+  int32_t n_drafts;
+  int32_t max_draft;         /* 0 .. 1024 */
+  int64_t n_vocab;
+  int32_t* n_accept;
+  int32_t* out_ids;
+  int32_t* err;
+} NhVerifyDrafts;
+int nh_verify_drafts(const NhVerifyDrafts* d, void* stream);
 
 /* ---- standalone forms used by the parity tests ---- */
 

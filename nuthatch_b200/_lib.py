@@ -40,6 +40,22 @@ class NhMoeLayer(C.Structure):
                 ("dump_offset", i64), ("scratch", vp)]
 
 
+class NhPagedKv(C.Structure):
+    _fields_ = [("k_codes", vp), ("v_codes", vp), ("k_scales", vp), ("v_scales", vp), ("n_pages", i32),
+                ("page_size", i32), ("n_head_kv", i32), ("head_dim", i32)]
+
+
+class NhPagedRows(C.Structure):
+    _fields_ = [("n_seq", i32), ("max_rows", i32), ("n_rows", i32), ("max_blocks", i32), ("row_off", vp),
+                ("pos0", vp), ("page_table", vp), ("err", vp)]
+
+
+class NhVerifyDrafts(C.Structure):
+    _fields_ = [("target", vp), ("target_stride", i64), ("draft", vp), ("draft_stride", i64), ("draft_ids", vp),
+                ("draft_off", vp), ("u_accept", vp), ("u_pick", vp), ("n_seq", i32), ("n_drafts", i32),
+                ("max_draft", i32), ("n_vocab", i64), ("n_accept", vp), ("out_ids", vp), ("err", vp)]
+
+
 # name -> (restype, argtypes)
 SIGNATURES = {
     # nh_api.h
@@ -153,6 +169,11 @@ SIGNATURES = {
                                             C.c_int, vp, vp]),
     "nh_batch_router_trace": (C.c_int, [vp, vp, C.c_int, i64, C.c_int, C.c_int, C.c_int, vp, vp, vp, vp, C.c_int,
                                         C.c_int, C.c_int, vp]),
+    "nh_paged_append": (C.c_int, [P(NhPagedKv), P(NhPagedRows), vp, i64, vp, i64, vp, i64, vp, vp, f32, C.c_int, vp,
+                                  C.c_int, vp, vp]),
+    "nh_paged_attention": (C.c_int, [P(NhPagedKv), P(NhPagedRows), vp, C.c_int, f32, C.c_int, C.c_int, vp, vp]),
+    "nh_paged_read": (C.c_int, [P(NhPagedKv), P(NhPagedRows), i32, vp, vp, vp]),
+    "nh_verify_drafts": (C.c_int, [P(NhVerifyDrafts), vp]),
     "nh_gemv": (C.c_int, [vp, vp, i32, i64, i64, vp, vp, f32, vp, vp]),
     "nh_quantize_q8k": (C.c_int, [vp, i64, vp, vp]),
     "nh_dequantize": (C.c_int, [vp, i32, i64, i64, vp, vp]),

@@ -1,60 +1,415 @@
-// Attention over the paged 8-bit K/V cache (nh_paged_attention).
+// Attention over the paged 8-bit K/V cache for few rows a sequence: decode
+// positions and drafted ones (nh_paged_attention's split form).
 //
-// The simplest right form: a warp per (row, head), lanes over the head's
-// dimensions, one position after the other with the running maximum and sum of
-// the softmax.
-#include "common.cuh"
-#include "paged.cuh"
+// What bounds it: every cached byte is read once, so the copy rate of HBM.  A
+// CTA takes up to 8 or 16 queries of one (sequence, KV head) and a contiguous
+// part of the positions; a cluster's CTAs split the positions and join their
+// (maximum, sum, weighted values) through distributed shared memory in rank
+// order.  A warp takes units of 16 positions, always inside one page: the codes
+// go from global memory straight into the operand layout of mma.m16n8k16 (both
+// the dimensions of K and those of V may be permuted freely, so each lane loads
+// whole 16-byte pieces), and the next unit's loads are issued as soon as the
+// registers are free.  The score accumulators are the weights' operand layout,
+// so nothing is shuffled between the two products.
+//   8 queries: rows 0-7 of the A operand are the high parts, 8-15 the low ones.
+//   16 queries: two A operands (the query's wait in shared memory), the codes'
+//   conversion shared by twice the queries.
+#include <cooperative_groups.h>
+
+#include "paged_attention.cuh"
+
+namespace cg = cooperative_groups;
 
 namespace nh {
 
 namespace {
 
-struct PagedAttnArgs {
-  PagedKv kv;
-  PagedRows rows;
-  const float* q;
-  float* out;
-  int n_head, group, window, n_sink;
-  float scale;
+constexpr int kSplitWarps = 4;
+constexpr int kSplitThreads = kSplitWarps * 32;
+constexpr int kUnit = 16;  // positions of one warp step
+
+__device__ __forceinline__ void mma_f16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                        uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};\n"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+// N consecutive 32-bit words through L2, in the widest pieces their alignment
+// (4 * N bytes, at most 16) allows.
+template <int N>
+__device__ __forceinline__ void load_words(const uint8_t* p, uint32_t* w) {
+  if constexpr (N % 4 == 0) {
+#pragma unroll
+    for (int i = 0; i < N / 4; ++i) {
+      const uint4 x = __ldcg(reinterpret_cast<const uint4*>(p) + i);
+      w[4 * i] = x.x;
+      w[4 * i + 1] = x.y;
+      w[4 * i + 2] = x.z;
+      w[4 * i + 3] = x.w;
+    }
+  } else if constexpr (N % 2 == 0) {
+#pragma unroll
+    for (int i = 0; i < N / 2; ++i) {
+      const uint2 x = __ldcg(reinterpret_cast<const uint2*>(p) + i);
+      w[2 * i] = x.x;
+      w[2 * i + 1] = x.y;
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < N; ++i) w[i] = __ldcg(reinterpret_cast<const uint32_t*>(p) + i);
+  }
+}
+
+template <int HD, int NQ>
+struct SplitShared {
+  float o[kSplitWarps][NQ][HD];  // [0] holds the CTA's joined values after the join
+  float m[kSplitWarps][NQ], l[kSplitWarps][NQ];
+  float cm[NQ], cl[NQ];
+  uint4 qa[NQ == 16 ? HD / 16 : 1][2][32];  // A operands of the 16-query form: high, low
 };
 
-__global__ void __launch_bounds__(32) paged_attention_kernel(const PagedAttnArgs p) {
+// Unit `i` of the visible ones: the sinks' units, then those from `lo` on.
+struct Units {
+  int n_sink, lo, n;
+  __device__ __forceinline__ int at(int i) const { return i < n_sink ? i : i - n_sink + lo; }
+};
+
+template <int HD, int NQ>
+__global__ void __launch_bounds__(kSplitThreads, NQ == 8 ? 3 : 2) paged_split_kernel(const PagedAttnArgs p) {
+  constexpr int KS = HD / 16;                    // k-steps of the score product
+  constexpr int KV = HD % 64 == 0 ? 16 : 8;      // contiguous bytes of K a lane loads at once
+  constexpr int KW = KV / 4, KN = HD / (4 * KV);  // words of such a piece, pieces a row
+  constexpr int VW = HD / 32;                    // words of V a lane loads a row
+  constexpr int QT = NQ / 8;                     // queries a lane holds scores of
+  extern __shared__ __align__(16) uint8_t split_smem[];
+  auto& sh = *reinterpret_cast<SplitShared<HD, NQ>*>(split_smem);
+  cg::cluster_group cluster = cg::this_cluster();
+  const int rank = static_cast<int>(cluster.block_rank()), nrank = static_cast<int>(cluster.num_blocks());
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
+  const int s = blockIdx.z, kh = static_cast<int>(blockIdx.y) % p.kv.n_kv, q0 = static_cast<int>(blockIdx.y) / p.kv.n_kv * NQ;
+  const int page = p.kv.page, lg = p.kv.page_log2;
   pdl_wait();
   pdl_trigger();
-  const int r = blockIdx.x, h = blockIdx.y, lane = threadIdx.x, hd = p.kv.hd, per = hd / 32, page = p.kv.page;
-  const int s = seq_of_row(p.rows, r);
-  if (s < 0) return;
   const SeqRows sq = seq_rows(p.rows, s, static_cast<int64_t>(p.rows.max_blocks) * page);
-  if (sq.n < 0) {
-    if (lane == 0) paged_error(p.rows);
-    return;
+  if (sq.n < 0 && blockIdx.y == 0 && rank == 0 && tid == 0) paged_error(p.rows);
+  const int n_q = sq.n * p.group;  // query j: row j / group, head kh * group + j % group
+  if (n_q <= q0 || n_q > p.few) return;  // every CTA of the cluster alike
+  const int nq = min(NQ, n_q - q0);
+
+  // Positions that any of these queries sees.
+  const int first_pos = sq.p0 + q0 / p.group, last_pos = sq.p0 + (q0 + nq - 1) / p.group;
+  Units un{0, 0, 0};
+  if (p.window > 0) {
+    un.lo = max(0, first_pos - p.window + 1) / kUnit;
+    un.n_sink = min((min(p.n_sink, last_pos + 1) + kUnit - 1) / kUnit, un.lo);
   }
-  const int pos = sq.p0 + (r - sq.r0), kh = h / p.group;
-  const float* q = p.q + (static_cast<int64_t>(r) * p.n_head + h) * hd + lane * per;
-  float qv[4], acc[4] = {0.f, 0.f, 0.f, 0.f}, m = -INFINITY, l = 0.f;
-  for (int i = 0; i < per; ++i) qv[i] = q[i] * p.scale;
-  for (int t = 0; t <= pos; ++t) {
-    if (p.window > 0 && t <= pos - p.window && t >= p.n_sink) t = pos - p.window + 1;
-    const int pg = p.rows.page_table[static_cast<int64_t>(s) * p.rows.max_blocks + (t >> p.kv.page_log2)];
-    if (pg < 0 || pg >= p.kv.n_pages) {
-      if (lane == 0) paged_error(p.rows);
-      continue;
+  un.n = un.n_sink + last_pos / kUnit + 1 - un.lo;
+  const int u0 = static_cast<int>(static_cast<int64_t>(un.n) * rank / nrank);
+  const int u1 = static_cast<int>(static_cast<int64_t>(un.n) * (rank + 1) / nrank);
+
+  // The query's operand: word w of lane t holds dimensions dim(w) .. dim(w)+3.
+  auto dim = [&](int w) { return (w / KW) * (4 * KV) + t * KV + (w % KW) * 4; };
+  uint32_t qa[NQ == 8 ? KS : 1][4];
+  float fq[QT], hq[QT];
+  int pos[QT];
+#pragma unroll
+  for (int k = 0; k < QT; ++k) {
+    const int j = q0 + g + 8 * k;
+    const bool ok = g + 8 * k < nq;
+    const int row = sq.r0 + (ok ? j / p.group : 0), head = kh * p.group + (ok ? j % p.group : 0);
+    pos[k] = ok ? sq.p0 + j / p.group : -1;
+    const float* q = p.q + (static_cast<int64_t>(row) * p.n_head + head) * HD;
+    float4 x[KS];
+    float top = 0.f;
+#pragma unroll
+    for (int w = 0; w < KS; ++w) {
+      x[w] = ok ? __ldcg(reinterpret_cast<const float4*>(q + dim(w))) : make_float4(0.f, 0.f, 0.f, 0.f);
+      top = fmaxf(top, fmaxf(fmaxf(fabsf(x[w].x), fabsf(x[w].y)), fmaxf(fabsf(x[w].z), fabsf(x[w].w))));
     }
-    const int64_t at = static_cast<int64_t>(pg) * p.kv.n_kv + kh, off = (at * page + (t & (page - 1))) * hd + lane * per;
-    const float ks = p.kv.k_scales[at], vs = p.kv.v_scales[at];
-    float d = 0.f;
-    for (int i = 0; i < per; ++i) d += qv[i] * (static_cast<float>(p.kv.k_codes[off + i]) - 127.5f);
-    const float x = warp_sum(d) * ks, mn = fmaxf(m, x), f = expf(m - mn), w = expf(x - mn);
-    m = mn;
-    l = l * f + w;
-    for (int i = 0; i < per; ++i) acc[i] = acc[i] * f + w * vs * (static_cast<float>(p.kv.v_codes[off + i]) - 127.5f);
+    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+    // The largest magnitude goes to [2^13, 2^14).
+    const int e = min(max(exponent_of(top), -100), 126);
+    const float up = pow2i(13 - e);
+    float sum = 0.f;
+#pragma unroll
+    for (int w = 0; w < KS; ++w) {
+      uint32_t h0, l0, h1, l1;
+      split2(x[w].x * up, x[w].y * up, h0, l0);
+      split2(x[w].z * up, x[w].w * up, h1, l1);
+      sum += (x[w].x * up + x[w].y * up) + (x[w].z * up + x[w].w * up);
+      if constexpr (NQ == 8) {
+        qa[w][0] = h0;
+        qa[w][1] = l0;
+        qa[w][2] = h1;
+        qa[w][3] = l1;
+      } else if (warp == 0) {
+        uint32_t* hi = reinterpret_cast<uint32_t*>(&sh.qa[w][0][lane]);
+        uint32_t* lo = reinterpret_cast<uint32_t*>(&sh.qa[w][1][lane]);
+        hi[k] = h0;
+        hi[2 + k] = h1;
+        lo[k] = l0;
+        lo[2 + k] = l1;
+      }
+    }
+    sum += __shfl_xor_sync(0xffffffffu, sum, 1);
+    sum += __shfl_xor_sync(0xffffffffu, sum, 2);
+    hq[k] = 0.5f * sum;
+    fq[k] = p.scale * kLog2e * pow2i(e - 13);
   }
-  float* o = p.out + (static_cast<int64_t>(r) * p.n_head + h) * hd + lane * per;
-  for (int i = 0; i < per; ++i) o[i] = l > 0.f ? acc[i] / l : 0.f;
+  if constexpr (NQ == 16) __syncthreads();
+
+  float o[HD / 8][4];
+#pragma unroll
+  for (int i = 0; i < HD / 8; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
+  float m[QT], l[QT], b[QT];  // running maximum; sum of the weights; sum of the weights in units of the values
+#pragma unroll
+  for (int k = 0; k < QT; ++k) {
+    m[k] = -INFINITY;
+    l[k] = b[k] = 0.f;
+  }
+  int eref = -200;  // the accumulators are in units of 2^(eref - kWeightShift)
+
+  const int32_t* table = p.rows.page_table + static_cast<int64_t>(s) * p.rows.max_blocks;
+  const int64_t head_bytes = static_cast<int64_t>(page) * HD;
+  uint32_t kw[2][KS], vw[4][VW];
+  float ks, vs;
+  auto page_of = [&](int i) { return i < u1 ? __ldcg(table + ((un.at(i) * kUnit) >> lg)) : 0; };
+  // A page out of range reads page 0 and hides its positions.
+  auto load_k = [&](int i, int pg) {
+    const int64_t at = static_cast<int64_t>(pg) * p.kv.n_kv + kh;
+    const uint8_t* k0 = p.kv.k_codes + at * head_bytes + ((un.at(i) * kUnit) & (page - 1)) * HD + g * HD + t * KV;
+#pragma unroll
+    for (int j = 0; j < 2; ++j)
+#pragma unroll
+      for (int c = 0; c < KN; ++c) load_words<KW>(k0 + j * 8 * HD + c * 4 * KV, &kw[j][c * KW]);
+    ks = __ldcg(p.kv.k_scales + at);
+    vs = __ldcg(p.kv.v_scales + at);
+  };
+  auto load_v = [&](int i, int pg) {
+    const int64_t at = static_cast<int64_t>(pg) * p.kv.n_kv + kh;
+    const uint8_t* v0 = p.kv.v_codes + at * head_bytes + ((un.at(i) * kUnit) & (page - 1)) * HD + 2 * t * HD + g * VW * 4;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) load_words<VW>(v0 + ((j & 1) + (j >> 1) * 8) * HD, vw[j]);
+  };
+  auto known = [&](int pg) { return pg >= 0 && pg < p.kv.n_pages; };
+
+  int i = u0 + warp;
+  int pg = page_of(i);
+  bool here = known(pg), lost = false;
+  if (i < u1) {
+    load_k(i, here ? pg : 0);
+    load_v(i, here ? pg : 0);
+  }
+  int pg_next = page_of(i + kSplitWarps);
+  for (; i < u1; i += kSplitWarps) {
+    const int t0 = un.at(i) * kUnit;
+    const bool seen_here = here;
+    lost |= !here;
+    const float k_scale = ks, v_scale = vs;
+    float c[2][4];
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      c[j][0] = c[j][1] = c[j][2] = c[j][3] = 0.f;
+#pragma unroll
+      for (int w = 0; w < KS; ++w) {
+        const uint32_t b0 = codes_lo(kw[j][w]), b1 = codes_hi(kw[j][w]);
+        if constexpr (NQ == 8) {
+          mma_f16(c[j], qa[w][0], qa[w][1], qa[w][2], qa[w][3], b0, b1);
+        } else {
+          const uint4 hi = sh.qa[w][0][lane], lo = sh.qa[w][1][lane];
+          mma_f16(c[j], hi.x, hi.y, hi.z, hi.w, b0, b1);
+          mma_f16(c[j], lo.x, lo.y, lo.z, lo.w, b0, b1);
+        }
+      }
+    }
+    const bool more = i + kSplitWarps < u1;
+    here = known(pg_next);
+    const int pg_load = here ? pg_next : 0;
+    if (more) load_k(i + kSplitWarps, pg_load);
+    pg_next = page_of(i + 2 * kSplitWarps);
+
+    // Scores of this lane's queries at positions t0 + 8 j + 2 t + e.
+    float x[QT][4], top[QT];
+    bool grew = false;
+#pragma unroll
+    for (int k = 0; k < QT; ++k) {
+      const float f = fq[k] * k_scale;
+      top[k] = m[k];
+#pragma unroll
+      for (int j = 0; j < 2; ++j)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const int tk = t0 + 8 * j + 2 * t + e;
+          const float d = NQ == 8 ? c[j][e] + c[j][e + 2] : c[j][2 * k + e];
+          const bool see = seen_here && tk <= pos[k] && (p.window == 0 || tk > pos[k] - p.window || tk < p.n_sink);
+          x[k][2 * j + e] = see ? (d + hq[k]) * f : -INFINITY;
+          top[k] = fmaxf(top[k], x[k][2 * j + e]);
+        }
+      top[k] = fmaxf(top[k], __shfl_xor_sync(0xffffffffu, top[k], 1));
+      top[k] = fmaxf(top[k], __shfl_xor_sync(0xffffffffu, top[k], 2));
+      grew |= top[k] > m[k];
+    }
+    const int ev = seen_here ? exponent_of(v_scale) : eref;
+    // Rarely after the first units: a larger score, or a larger scale of V.
+    if (__any_sync(0xffffffffu, grew) || ev > eref) {
+      const int en = max(eref, ev);
+      const float fe = pow2i(max(eref - en, -200));
+#pragma unroll
+      for (int k = 0; k < QT; ++k) {
+        const float a = m[k] == -INFINITY ? 0.f : exp2_fast(m[k] - top[k]);
+        m[k] = top[k];
+        l[k] *= a;
+        b[k] *= a * fe;
+#pragma unroll
+        for (int n = 0; n < HD / 8; ++n) {
+          if constexpr (NQ == 8) {
+            o[n][0] *= a * fe;
+            o[n][1] *= a * fe;
+            o[n][2] *= a * fe;
+            o[n][3] *= a * fe;
+          } else {
+            o[n][2 * k] *= a * fe;
+            o[n][2 * k + 1] *= a * fe;
+          }
+        }
+      }
+      eref = en;
+    }
+    const float fw = pow2i(ev - eref + kWeightShift);
+    uint32_t hi[QT][2], lo[QT][2];
+#pragma unroll
+    for (int k = 0; k < QT; ++k) {
+      const float base = m[k] == -INFINITY ? 0.f : m[k];
+      float w[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        w[e] = exp2_fast(x[k][e] - base);
+        l[k] += w[e];
+        w[e] *= fw;
+        b[k] += w[e];
+      }
+      split2(w[0], w[1], hi[k][0], lo[k][0]);
+      split2(w[2], w[3], hi[k][1], lo[k][1]);
+    }
+#pragma unroll
+    for (int w = 0; w < VW; ++w) {
+      const uint32_t a01 = __byte_perm(vw[0][w], vw[1][w], 0x5140), a23 = __byte_perm(vw[0][w], vw[1][w], 0x7362);
+      const uint32_t b01 = __byte_perm(vw[2][w], vw[3][w], 0x5140), b23 = __byte_perm(vw[2][w], vw[3][w], 0x7362);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const uint32_t v0 = e & 1 ? codes_hi(e < 2 ? a01 : a23) : codes_lo(e < 2 ? a01 : a23);
+        const uint32_t v1 = e & 1 ? codes_hi(e < 2 ? b01 : b23) : codes_lo(e < 2 ? b01 : b23);
+        if constexpr (NQ == 8) {
+          mma_f16(o[4 * w + e], hi[0][0], lo[0][0], hi[0][1], lo[0][1], v0, v1);
+        } else {
+          mma_f16(o[4 * w + e], hi[0][0], hi[1][0], hi[0][1], hi[1][1], v0, v1);
+          mma_f16(o[4 * w + e], lo[0][0], lo[1][0], lo[0][1], lo[1][1], v0, v1);
+        }
+      }
+    }
+    if (more) load_v(i + kSplitWarps, pg_load);
+  }
+  if (lost && lane == 0) paged_error(p.rows);
+
+  // This warp's values in their own units, then the CTA's and the cluster's.
+  const float unit = pow2i(max(eref, -126));
+#pragma unroll
+  for (int k = 0; k < QT; ++k) {
+    l[k] += __shfl_xor_sync(0xffffffffu, l[k], 1);
+    l[k] += __shfl_xor_sync(0xffffffffu, l[k], 2);
+    b[k] += __shfl_xor_sync(0xffffffffu, b[k], 1);
+    b[k] += __shfl_xor_sync(0xffffffffu, b[k], 2);
+    if (t == 0) {
+      sh.m[warp][g + 8 * k] = m[k];
+      sh.l[warp][g + 8 * k] = l[k];
+    }
+#pragma unroll
+    for (int n = 0; n < HD / 8; ++n)
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const float v = NQ == 8 ? o[n][e] + o[n][e + 2] : o[n][2 * k + e];
+        sh.o[warp][g + 8 * k][(2 * t + e) * VW * 4 + n] = (v + 0.5f * b[k]) * pow2i(-kWeightShift) * unit;
+      }
+  }
+  __syncthreads();
+  for (int j = tid; j < NQ; j += kSplitThreads) {
+    float top = -INFINITY, sum = 0.f;
+    for (int w = 0; w < kSplitWarps; ++w) top = fmaxf(top, sh.m[w][j]);
+    for (int w = 0; w < kSplitWarps; ++w) {
+      const float a = sh.m[w][j] == -INFINITY ? 0.f : exp2_fast(sh.m[w][j] - top);
+      sh.m[w][j] = a;  // from here on the warp's factor
+      sum += a * sh.l[w][j];
+    }
+    sh.cm[j] = top;
+    sh.cl[j] = sum;
+  }
+  __syncthreads();
+  for (int j = tid; j < nq * HD; j += kSplitThreads) {
+    const int q = j / HD, d = j % HD;
+    float v = 0.f;
+#pragma unroll
+    for (int w = 0; w < kSplitWarps; ++w) v += sh.m[w][q] * sh.o[w][q][d];
+    sh.o[0][q][d] = v;
+  }
+  if (nrank > 1)
+    cluster.sync();
+  else
+    __syncthreads();
+  const int per = (nq * HD + nrank - 1) / nrank;
+  for (int j = rank * per + tid; j < min((rank + 1) * per, nq * HD); j += kSplitThreads) {
+    const int q = j / HD, d = j % HD, qi = q0 + q;
+    float top = -INFINITY, sum = 0.f, v = 0.f;
+    for (int r = 0; r < nrank; ++r) top = fmaxf(top, cluster.map_shared_rank(sh.cm, r)[q]);
+    for (int r = 0; r < nrank; ++r) {
+      const float mr = cluster.map_shared_rank(sh.cm, r)[q];
+      const float a = mr == -INFINITY ? 0.f : exp2_fast(mr - top);
+      sum += a * cluster.map_shared_rank(sh.cl, r)[q];
+      v += a * cluster.map_shared_rank(&sh.o[0][0][0], r)[j];
+    }
+    const int row = sq.r0 + qi / p.group, head = kh * p.group + qi % p.group;
+    p.out[(static_cast<int64_t>(row) * p.n_head + head) * HD + d] = sum == 0.f ? 0.f : v / sum;
+  }
+  if (nrank > 1) cluster.sync();  // no CTA leaves while another reads its part
+}
+
+template <int HD, int NQ>
+int launch_split(const PagedAttnArgs& p, int groups, int ranks, cudaStream_t s) {
+  static SmemLimit configured;
+  const size_t smem = sizeof(SplitShared<HD, NQ>);
+  if (!ensure_smem(paged_split_kernel<HD, NQ>, smem, configured)) return NH_E_CUDA;
+  return launch_cluster(paged_split_kernel<HD, NQ>, dim3(ranks, p.kv.n_kv * groups, p.rows.n_seq), dim3(kSplitThreads),
+                        ranks, smem, s, p);
+}
+
+template <int HD>
+int launch_split_hd(const PagedAttnArgs& p, cudaStream_t s) {
+  const int64_t most = std::min<int64_t>(p.few, static_cast<int64_t>(p.rows.max_rows) * p.group);
+  const int nq = most <= 8 ? 8 : 16, groups = static_cast<int>((most + nq - 1) / nq);
+  if (static_cast<int64_t>(p.kv.n_kv) * groups > 65535) return NH_E_ARG;
+  const int64_t items = static_cast<int64_t>(p.rows.n_seq) * p.kv.n_kv * groups;
+  const int64_t units = static_cast<int64_t>(p.rows.max_blocks) * p.kv.page / kUnit;
+  int ranks = 1;
+  while (ranks < 8 && items * ranks < 4 * device_sm_count() && units > 2 * kSplitWarps * ranks) ranks *= 2;
+  return nq == 8 ? launch_split<HD, 8>(p, groups, ranks, s) : launch_split<HD, 16>(p, groups, ranks, s);
 }
 
 }  // namespace
+
+int launch_paged_split(const PagedAttnArgs& p, cudaStream_t s) {
+  switch (p.kv.hd) {
+    case 32:
+      return launch_split_hd<32>(p, s);
+    case 64:
+      return launch_split_hd<64>(p, s);
+    case 96:
+      return launch_split_hd<96>(p, s);
+    default:
+      return launch_split_hd<128>(p, s);
+  }
+}
 
 }  // namespace nh
 
@@ -68,7 +423,7 @@ extern "C" int nh_paged_attention(const NhPagedKv* kv, const NhPagedRows* rows, 
   if (qr == nullptr || out == nullptr || !paged_aligned(qr) || !paged_aligned(out) || n_head <= 0 || n_head > 65535 ||
       n_head % p.kv.n_kv != 0 || window < 0 || n_sink < 0)
     return NH_E_ARG;
-  if (p.rows.n_rows == 0) return NH_OK;
+  if (p.rows.max_rows == 0) return NH_OK;
   p.q = qr;
   p.out = out;
   p.n_head = n_head;
@@ -76,6 +431,6 @@ extern "C" int nh_paged_attention(const NhPagedKv* kv, const NhPagedRows* rows, 
   p.window = window;
   p.n_sink = n_sink;
   p.scale = kq_scale;
-  return launch_pdl(paged_attention_kernel, dim3(p.rows.n_rows, n_head), dim3(32), 0,
-                    static_cast<cudaStream_t>(stream), p);
+  p.few = INT32_MAX;
+  return launch_paged_split(p, static_cast<cudaStream_t>(stream));
 }

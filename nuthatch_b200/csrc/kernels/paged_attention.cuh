@@ -1,0 +1,60 @@
+// What the two forms of the paged attention share: arguments, the visible
+// range, exact 8-bit codes as f16 operands and the two-part split of f32
+// factors.
+//
+// Arithmetic.  A code u stands for (c + 1/2) * s with c = u - 128 and s a power
+// of two, so c is exact in f16.  A query row is scaled by a power of two and
+// split into two f16 parts (22 bits of it), likewise a softmax weight; both
+// parts' products are exact and the tensor cores add them up in f32.  The half
+// codes come in apart: 1/2 * sum(q) per score, 1/2 * sum(w) per output.
+#pragma once
+
+#include "common.cuh"
+#include "paged.cuh"
+
+namespace nh {
+
+struct PagedAttnArgs {
+  PagedKv kv;
+  PagedRows rows;
+  const float* q;
+  float* out;
+  int n_head, group, window, n_sink;
+  float scale;
+  int few;  // sequences of at most this many queries a KV head (rows x group) go to the split form
+};
+
+constexpr float kLog2e = 1.44269504088896340736f;
+constexpr int kWeightShift = 15;  // a weight in [0, 1] times 2^15 keeps 22 bits in two f16 parts down to 2^-29
+
+// 2^e as a float, 0 below the normal range; e <= 127.
+__device__ __forceinline__ float pow2i(int e) { return e < -126 ? 0.f : __int_as_float((e + 127) << 23); }
+__device__ __forceinline__ int exponent_of(float s) { return ((__float_as_int(s) >> 23) & 255) - 127; }
+
+// Bytes 0, 1 (or 2, 3) of w as two f16 codes c = u - 128: 0x64uu is 1024 + u.
+__device__ __forceinline__ uint32_t codes_f16(uint32_t w, uint32_t sel) {
+  const uint32_t x = __byte_perm(w, 0x64646464u, sel);
+  const __half2 r = __hsub2(*reinterpret_cast<const __half2*>(&x), __half2half2(__ushort_as_half(0x6480)));
+  return *reinterpret_cast<const uint32_t*>(&r);
+}
+__device__ __forceinline__ uint32_t codes_lo(uint32_t w) { return codes_f16(w, 0x4140); }
+__device__ __forceinline__ uint32_t codes_hi(uint32_t w) { return codes_f16(w, 0x4342); }
+
+// x and y as f16 pairs hi + lo.
+__device__ __forceinline__ void split2(float x, float y, uint32_t& hi, uint32_t& lo) {
+  const __half2 h = __floats2half2_rn(x, y);
+  const float2 b = __half22float2(h);
+  const __half2 l = __floats2half2_rn(x - b.x, y - b.y);
+  hi = *reinterpret_cast<const uint32_t*>(&h);
+  lo = *reinterpret_cast<const uint32_t*>(&l);
+}
+
+__device__ __forceinline__ float exp2_fast(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+int launch_paged_split(const PagedAttnArgs& p, cudaStream_t s);
+
+}  // namespace nh

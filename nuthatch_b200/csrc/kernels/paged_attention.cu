@@ -2,16 +2,19 @@
 // positions and drafted ones (nh_paged_attention's split form).
 //
 // What bounds it: every cached byte is read once, so the copy rate of HBM.  A
-// CTA takes up to 8 or 16 queries of one (sequence, KV head) and a contiguous
+// CTA takes up to 4, 8 or 16 queries of one (sequence, KV head) and a contiguous
 // part of the positions; a cluster's CTAs split the positions and join their
 // (maximum, sum, weighted values) through distributed shared memory in rank
 // order.  A warp takes units of 16 positions, always inside one page: the codes
 // go from global memory straight into the operand layout of mma.m16n8k16 (both
 // the dimensions of K and those of V may be permuted freely, so each lane loads
 // whole 16-byte pieces), and the next unit's loads are issued as soon as the
-// registers are free.  The score accumulators are the weights' operand layout,
-// so nothing is shuffled between the two products.
-//   8 queries: rows 0-7 of the A operand are the high parts, 8-15 the low ones.
+// registers are free.
+//   4 queries: the codes are the A operand, the queries' (and weights') high
+//   and low parts the 8 columns of B; half the products and accumulators of the
+//   next form, four shuffles to bring the weights into place.
+//   8 queries: rows 0-7 of the A operand are the high parts, 8-15 the low ones,
+//   the codes are B; the score accumulators are the weights' operand layout.
 //   16 queries: two A operands (the query's wait in shared memory), the codes'
 //   conversion shared by twice the queries.
 #include <cooperative_groups.h>
@@ -77,12 +80,14 @@ struct Units {
 };
 
 template <int HD, int NQ>
-__global__ void __launch_bounds__(kSplitThreads, NQ == 8 ? 3 : 2) paged_split_kernel(const PagedAttnArgs p) {
+__global__ void __launch_bounds__(kSplitThreads, NQ == 4 ? 4 : NQ == 8 ? 3 : 2) paged_split_kernel(const PagedAttnArgs p) {
   constexpr int KS = HD / 16;                    // k-steps of the score product
   constexpr int KV = HD % 64 == 0 ? 16 : 8;      // contiguous bytes of K a lane loads at once
   constexpr int KW = KV / 4, KN = HD / (4 * KV);  // words of such a piece, pieces a row
   constexpr int VW = HD / 32;                    // words of V a lane loads a row
-  constexpr int QT = NQ / 8;                     // queries a lane holds scores of
+  constexpr int QT = NQ == 16 ? 2 : 1;           // queries a lane holds scores of
+  constexpr int ST = NQ == 4 ? 2 : 4;            // scores a lane holds of each, a unit
+  constexpr int ON = NQ == 4 ? HD / 16 : HD / 8;  // accumulator tiles
   extern __shared__ __align__(16) uint8_t split_smem[];
   auto& sh = *reinterpret_cast<SplitShared<HD, NQ>*>(split_smem);
   cg::cluster_group cluster = cg::this_cluster();
@@ -111,13 +116,14 @@ __global__ void __launch_bounds__(kSplitThreads, NQ == 8 ? 3 : 2) paged_split_ke
 
   // The query's operand: word w of lane t holds dimensions dim(w) .. dim(w)+3.
   auto dim = [&](int w) { return (w / KW) * (4 * KV) + t * KV + (w % KW) * 4; };
-  uint32_t qa[NQ == 8 ? KS : 1][4];
+  uint32_t qa[NQ <= 8 ? KS : 1][4];
   float fq[QT], hq[QT];
   int pos[QT];
 #pragma unroll
   for (int k = 0; k < QT; ++k) {
-    const int j = q0 + g + 8 * k;
-    const bool ok = g + 8 * k < nq;
+    const int jq = NQ == 4 ? g >> 1 : g + 8 * k;  // the query whose operand this lane holds
+    const int j = q0 + jq;
+    const bool ok = jq < nq;
     const int row = sq.r0 + (ok ? j / p.group : 0), head = kh * p.group + (ok ? j % p.group : 0);
     pos[k] = ok ? sq.p0 + j / p.group : -1;
     const float* q = p.q + (static_cast<int64_t>(row) * p.n_head + head) * HD;
@@ -140,7 +146,10 @@ __global__ void __launch_bounds__(kSplitThreads, NQ == 8 ? 3 : 2) paged_split_ke
       split2(x[w].x * up, x[w].y * up, h0, l0);
       split2(x[w].z * up, x[w].w * up, h1, l1);
       sum += (x[w].x * up + x[w].y * up) + (x[w].z * up + x[w].w * up);
-      if constexpr (NQ == 8) {
+      if constexpr (NQ == 4) {
+        qa[w][0] = g & 1 ? l0 : h0;
+        qa[w][1] = g & 1 ? l1 : h1;
+      } else if constexpr (NQ == 8) {
         qa[w][0] = h0;
         qa[w][1] = l0;
         qa[w][2] = h1;
@@ -158,12 +167,17 @@ __global__ void __launch_bounds__(kSplitThreads, NQ == 8 ? 3 : 2) paged_split_ke
     sum += __shfl_xor_sync(0xffffffffu, sum, 2);
     hq[k] = 0.5f * sum;
     fq[k] = p.scale * kLog2e * pow2i(e - 13);
+    if constexpr (NQ == 4) {  // scores: query t, whose operand lanes 8 t hold
+      hq[k] = __shfl_sync(0xffffffffu, hq[k], 8 * t);
+      fq[k] = __shfl_sync(0xffffffffu, fq[k], 8 * t);
+      pos[k] = __shfl_sync(0xffffffffu, pos[k], 8 * t);
+    }
   }
   if constexpr (NQ == 16) __syncthreads();
 
-  float o[HD / 8][4];
+  float o[ON][4];
 #pragma unroll
-  for (int i = 0; i < HD / 8; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
+  for (int i = 0; i < ON; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
   float m[QT], l[QT], b[QT];  // running maximum; sum of the weights; sum of the weights in units of the values
 #pragma unroll
   for (int k = 0; k < QT; ++k) {
@@ -209,20 +223,23 @@ __global__ void __launch_bounds__(kSplitThreads, NQ == 8 ? 3 : 2) paged_split_ke
     const bool seen_here = here;
     lost |= !here;
     const float k_scale = ks, v_scale = vs;
-    float c[2][4];
+    float c[2][4];  // two chains of products: of even and odd k-steps (4 queries), of positions 0-7 and 8-15 (others)
 #pragma unroll
-    for (int j = 0; j < 2; ++j) {
-      c[j][0] = c[j][1] = c[j][2] = c[j][3] = 0.f;
+    for (int j = 0; j < 2; ++j) c[j][0] = c[j][1] = c[j][2] = c[j][3] = 0.f;
 #pragma unroll
-      for (int w = 0; w < KS; ++w) {
-        const uint32_t b0 = codes_lo(kw[j][w]), b1 = codes_hi(kw[j][w]);
-        if constexpr (NQ == 8) {
-          mma_f16(c[j], qa[w][0], qa[w][1], qa[w][2], qa[w][3], b0, b1);
-        } else {
-          const uint4 hi = sh.qa[w][0][lane], lo = sh.qa[w][1][lane];
-          mma_f16(c[j], hi.x, hi.y, hi.z, hi.w, b0, b1);
-          mma_f16(c[j], lo.x, lo.y, lo.z, lo.w, b0, b1);
-        }
+    for (int w = 0; w < KS; ++w) {
+      const uint32_t a0 = codes_lo(kw[0][w]), a1 = codes_hi(kw[0][w]), b0 = codes_lo(kw[1][w]), b1 = codes_hi(kw[1][w]);
+      if constexpr (NQ == 4) {
+        mma_f16(c[w & 1], a0, b0, a1, b1, qa[w][0], qa[w][1]);
+      } else if constexpr (NQ == 8) {
+        mma_f16(c[0], qa[w][0], qa[w][1], qa[w][2], qa[w][3], a0, a1);
+        mma_f16(c[1], qa[w][0], qa[w][1], qa[w][2], qa[w][3], b0, b1);
+      } else {
+        const uint4 hi = sh.qa[w][0][lane], lo = sh.qa[w][1][lane];
+        mma_f16(c[0], hi.x, hi.y, hi.z, hi.w, a0, a1);
+        mma_f16(c[1], hi.x, hi.y, hi.z, hi.w, b0, b1);
+        mma_f16(c[0], lo.x, lo.y, lo.z, lo.w, a0, a1);
+        mma_f16(c[1], lo.x, lo.y, lo.z, lo.w, b0, b1);
       }
     }
     const bool more = i + kSplitWarps < u1;
@@ -231,25 +248,35 @@ __global__ void __launch_bounds__(kSplitThreads, NQ == 8 ? 3 : 2) paged_split_ke
     if (more) load_k(i + kSplitWarps, pg_load);
     pg_next = page_of(i + 2 * kSplitWarps);
 
-    // Scores of this lane's queries at positions t0 + 8 j + 2 t + e.
-    float x[QT][4], top[QT];
+    // Scores of this lane's queries: at positions t0 + g, t0 + g + 8 (4 queries), t0 + 8 j + 2 t + e (others).
+    const bool plain = seen_here && t0 + kUnit - 1 <= first_pos &&
+                       (p.window == 0 || t0 > last_pos - p.window || t0 + kUnit <= p.n_sink);  // all of them see all
+    float x[QT][ST], top[QT];
     bool grew = false;
 #pragma unroll
     for (int k = 0; k < QT; ++k) {
       const float f = fq[k] * k_scale;
+#pragma unroll
+      for (int e = 0; e < ST; ++e) {
+        const float d = NQ == 4   ? (c[0][2 * e] + c[1][2 * e]) + (c[0][2 * e + 1] + c[1][2 * e + 1])
+                        : NQ == 8 ? c[e >> 1][e & 1] + c[e >> 1][(e & 1) + 2]
+                                  : c[e >> 1][2 * k + (e & 1)];
+        x[k][e] = (d + hq[k]) * f;
+      }
+      if (!plain) {
+#pragma unroll
+        for (int e = 0; e < ST; ++e) {
+          const int tk = t0 + (NQ == 4 ? g + 8 * e : 8 * (e >> 1) + 2 * t + (e & 1));
+          if (!seen_here || tk > pos[k] || (p.window != 0 && tk <= pos[k] - p.window && tk >= p.n_sink))
+            x[k][e] = -INFINITY;
+        }
+      }
       top[k] = m[k];
 #pragma unroll
-      for (int j = 0; j < 2; ++j)
+      for (int e = 0; e < ST; ++e) top[k] = fmaxf(top[k], x[k][e]);
 #pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          const int tk = t0 + 8 * j + 2 * t + e;
-          const float d = NQ == 8 ? c[j][e] + c[j][e + 2] : c[j][2 * k + e];
-          const bool see = seen_here && tk <= pos[k] && (p.window == 0 || tk > pos[k] - p.window || tk < p.n_sink);
-          x[k][2 * j + e] = see ? (d + hq[k]) * f : -INFINITY;
-          top[k] = fmaxf(top[k], x[k][2 * j + e]);
-        }
-      top[k] = fmaxf(top[k], __shfl_xor_sync(0xffffffffu, top[k], 1));
-      top[k] = fmaxf(top[k], __shfl_xor_sync(0xffffffffu, top[k], 2));
+      for (int e = NQ == 4 ? 4 : 1; e <= (NQ == 4 ? 16 : 2); e <<= 1)
+        top[k] = fmaxf(top[k], __shfl_xor_sync(0xffffffffu, top[k], e));
       grew |= top[k] > m[k];
     }
     const int ev = seen_here ? exponent_of(v_scale) : eref;
@@ -264,8 +291,8 @@ __global__ void __launch_bounds__(kSplitThreads, NQ == 8 ? 3 : 2) paged_split_ke
         l[k] *= a;
         b[k] *= a * fe;
 #pragma unroll
-        for (int n = 0; n < HD / 8; ++n) {
-          if constexpr (NQ == 8) {
+        for (int n = 0; n < ON; ++n) {
+          if constexpr (NQ <= 8) {
             o[n][0] *= a * fe;
             o[n][1] *= a * fe;
             o[n][2] *= a * fe;
@@ -285,28 +312,45 @@ __global__ void __launch_bounds__(kSplitThreads, NQ == 8 ? 3 : 2) paged_split_ke
       const float base = m[k] == -INFINITY ? 0.f : m[k];
       float w[4];
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
+      for (int e = 0; e < ST; ++e) {
         w[e] = exp2_fast(x[k][e] - base);
         l[k] += w[e];
         w[e] *= fw;
         b[k] += w[e];
       }
+      if constexpr (NQ == 4) {
+        // Column g of B: query g / 2's weights at positions 2 t, 2 t + 1 and 8 further, from the lanes that hold them.
+        const int from = 8 * t + (g >> 1);
+        const float w0 = __shfl_sync(0xffffffffu, w[0], from), w1 = __shfl_sync(0xffffffffu, w[0], from + 4);
+        const float w2 = __shfl_sync(0xffffffffu, w[1], from), w3 = __shfl_sync(0xffffffffu, w[1], from + 4);
+        w[0] = w0;
+        w[1] = w1;
+        w[2] = w2;
+        w[3] = w3;
+      }
       split2(w[0], w[1], hi[k][0], lo[k][0]);
       split2(w[2], w[3], hi[k][1], lo[k][1]);
     }
+    const uint32_t b0 = g & 1 ? lo[0][0] : hi[0][0], b1 = g & 1 ? lo[0][1] : hi[0][1];  // 4 queries
 #pragma unroll
     for (int w = 0; w < VW; ++w) {
+      // Positions 2 t, 2 t + 1 (a) and 8 further (b) side by side, for dimensions 0, 1 and 2, 3 of the word.
       const uint32_t a01 = __byte_perm(vw[0][w], vw[1][w], 0x5140), a23 = __byte_perm(vw[0][w], vw[1][w], 0x7362);
       const uint32_t b01 = __byte_perm(vw[2][w], vw[3][w], 0x5140), b23 = __byte_perm(vw[2][w], vw[3][w], 0x7362);
+      const uint32_t va[4] = {codes_lo(a01), codes_hi(a01), codes_lo(a23), codes_hi(a23)};
+      const uint32_t vb[4] = {codes_lo(b01), codes_hi(b01), codes_lo(b23), codes_hi(b23)};
+      if constexpr (NQ == 4) {
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const uint32_t v0 = e & 1 ? codes_hi(e < 2 ? a01 : a23) : codes_lo(e < 2 ? a01 : a23);
-        const uint32_t v1 = e & 1 ? codes_hi(e < 2 ? b01 : b23) : codes_lo(e < 2 ? b01 : b23);
-        if constexpr (NQ == 8) {
-          mma_f16(o[4 * w + e], hi[0][0], lo[0][0], hi[0][1], lo[0][1], v0, v1);
-        } else {
-          mma_f16(o[4 * w + e], hi[0][0], hi[1][0], hi[0][1], hi[1][1], v0, v1);
-          mma_f16(o[4 * w + e], lo[0][0], lo[1][0], lo[0][1], lo[1][1], v0, v1);
+        for (int e = 0; e < 2; ++e) mma_f16(o[2 * w + e], va[2 * e], va[2 * e + 1], vb[2 * e], vb[2 * e + 1], b0, b1);
+      } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          if constexpr (NQ == 8) {
+            mma_f16(o[4 * w + e], hi[0][0], lo[0][0], hi[0][1], lo[0][1], va[e], vb[e]);
+          } else {
+            mma_f16(o[4 * w + e], hi[0][0], hi[1][0], hi[0][1], hi[1][1], va[e], vb[e]);
+            mma_f16(o[4 * w + e], lo[0][0], lo[1][0], lo[0][1], lo[1][1], va[e], vb[e]);
+          }
         }
       }
     }
@@ -318,20 +362,23 @@ __global__ void __launch_bounds__(kSplitThreads, NQ == 8 ? 3 : 2) paged_split_ke
   const float unit = pow2i(max(eref, -126));
 #pragma unroll
   for (int k = 0; k < QT; ++k) {
-    l[k] += __shfl_xor_sync(0xffffffffu, l[k], 1);
-    l[k] += __shfl_xor_sync(0xffffffffu, l[k], 2);
-    b[k] += __shfl_xor_sync(0xffffffffu, b[k], 1);
-    b[k] += __shfl_xor_sync(0xffffffffu, b[k], 2);
-    if (t == 0) {
-      sh.m[warp][g + 8 * k] = m[k];
-      sh.l[warp][g + 8 * k] = l[k];
+#pragma unroll
+    for (int e = NQ == 4 ? 4 : 1; e <= (NQ == 4 ? 16 : 2); e <<= 1) {
+      l[k] += __shfl_xor_sync(0xffffffffu, l[k], e);
+      b[k] += __shfl_xor_sync(0xffffffffu, b[k], e);
+    }
+    const int qk = NQ == 4 ? t : g + 8 * k;
+    if (NQ == 4 ? g == 0 : t == 0) {
+      sh.m[warp][qk] = m[k];
+      sh.l[warp][qk] = l[k];
     }
 #pragma unroll
-    for (int n = 0; n < HD / 8; ++n)
+    for (int n = 0; n < ON; ++n)
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
-        const float v = NQ == 8 ? o[n][e] + o[n][e + 2] : o[n][2 * k + e];
-        sh.o[warp][g + 8 * k][(2 * t + e) * VW * 4 + n] = (v + 0.5f * b[k]) * pow2i(-kWeightShift) * unit;
+        const float v = NQ == 4 ? o[n][2 * e] + o[n][2 * e + 1] : NQ == 8 ? o[n][e] + o[n][e + 2] : o[n][2 * k + e];
+        const int d = NQ == 4 ? g * VW * 4 + 2 * n + e : (2 * t + e) * VW * 4 + n;
+        sh.o[warp][qk][d] = (v + 0.5f * b[k]) * pow2i(-kWeightShift) * unit;
       }
   }
   __syncthreads();
@@ -387,13 +434,15 @@ int launch_split(const PagedAttnArgs& p, int groups, int ranks, cudaStream_t s) 
 template <int HD>
 int launch_split_hd(const PagedAttnArgs& p, cudaStream_t s) {
   const int64_t most = std::min<int64_t>(p.few, static_cast<int64_t>(p.rows.max_rows) * p.group);
-  const int nq = most <= 8 ? 8 : 16, groups = static_cast<int>((most + nq - 1) / nq);
+  const int nq = most <= 4 ? 4 : most <= 8 ? 8 : 16, groups = static_cast<int>((most + nq - 1) / nq);
   if (static_cast<int64_t>(p.kv.n_kv) * groups > 65535) return NH_E_ARG;
   const int64_t items = static_cast<int64_t>(p.rows.n_seq) * p.kv.n_kv * groups;
   const int64_t units = static_cast<int64_t>(p.rows.max_blocks) * p.kv.page / kUnit;
   int ranks = 1;
   while (ranks < 8 && items * ranks < 4 * device_sm_count() && units > 2 * kSplitWarps * ranks) ranks *= 2;
-  return nq == 8 ? launch_split<HD, 8>(p, groups, ranks, s) : launch_split<HD, 16>(p, groups, ranks, s);
+  return nq == 4   ? launch_split<HD, 4>(p, groups, ranks, s)
+         : nq == 8 ? launch_split<HD, 8>(p, groups, ranks, s)
+                   : launch_split<HD, 16>(p, groups, ranks, s);
 }
 
 }  // namespace

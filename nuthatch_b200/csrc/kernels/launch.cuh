@@ -120,6 +120,25 @@ int launch_pdl(void (*kern)(KArgs...), dim3 grid, dim3 block, size_t smem, cudaS
   return cudaLaunchKernelEx(&cfg, kern, std::forward<Args>(args)...) == cudaSuccess ? NH_OK : NH_E_CUDA;
 }
 
+// Whether one kernel may be launched in clusters of 16 (above the portable 8),
+// set once per device as SmemLimit is.
+struct WideCluster {
+  std::atomic<bool> set[SmemLimit::kMaxDevices];
+  WideCluster() {
+    for (auto& s : set) s.store(false, std::memory_order_relaxed);
+  }
+};
+
+template <typename Kern>
+bool ensure_wide_cluster(Kern k, WideCluster& rec) {
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= SmemLimit::kMaxDevices) return false;
+  if (rec.set[dev].load(std::memory_order_acquire)) return true;
+  if (cudaFuncSetAttribute(k, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) != cudaSuccess) return false;
+  rec.set[dev].store(true, std::memory_order_release);
+  return true;
+}
+
 // launch_pdl with thread-block clusters of `cluster` CTAs along x.
 template <typename... KArgs, typename... Args>
 int launch_cluster(void (*kern)(KArgs...), dim3 grid, dim3 block, int cluster, size_t smem, cudaStream_t s,

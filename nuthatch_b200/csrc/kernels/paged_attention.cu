@@ -5,11 +5,11 @@
 // CTA takes up to 4, 8 or 16 queries of one (sequence, KV head) and a contiguous
 // part of the positions; a cluster's CTAs split the positions and join their
 // (maximum, sum, weighted values) through distributed shared memory in rank
-// order.  A warp takes units of 16 positions, always inside one page: the codes
-// go from global memory straight into the operand layout of mma.m16n8k16 (both
-// the dimensions of K and those of V may be permuted freely, so each lane loads
-// whole 16-byte pieces), and the next unit's loads are issued as soon as the
-// registers are free.
+// order.  A warp takes units of 16 positions, always inside one page, through a
+// ring of stages of its own in shared memory (cp.async, no barrier between
+// warps), and reads them in the operand layout of mma.m16n8k16: both the
+// dimensions of K and those of V may be permuted freely, so each lane reads
+// whole 16-byte pieces.
 //   4 queries: the codes are the A operand, the queries' (and weights') high
 //   and low parts the 8 columns of B; half the products and accumulators of the
 //   next form, four shuffles to bring the weights into place.
@@ -39,14 +39,14 @@ __device__ __forceinline__ void mma_f16(float (&d)[4], uint32_t a0, uint32_t a1,
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
-// N consecutive 32-bit words through L2, in the widest pieces their alignment
-// (4 * N bytes, at most 16) allows.
+// N consecutive 32-bit words of shared memory, in the widest pieces their
+// alignment (4 * N bytes, at most 16) allows.
 template <int N>
 __device__ __forceinline__ void load_words(const uint8_t* p, uint32_t* w) {
   if constexpr (N % 4 == 0) {
 #pragma unroll
     for (int i = 0; i < N / 4; ++i) {
-      const uint4 x = __ldcg(reinterpret_cast<const uint4*>(p) + i);
+      const uint4 x = reinterpret_cast<const uint4*>(p)[i];
       w[4 * i] = x.x;
       w[4 * i + 1] = x.y;
       w[4 * i + 2] = x.z;
@@ -55,19 +55,39 @@ __device__ __forceinline__ void load_words(const uint8_t* p, uint32_t* w) {
   } else if constexpr (N % 2 == 0) {
 #pragma unroll
     for (int i = 0; i < N / 2; ++i) {
-      const uint2 x = __ldcg(reinterpret_cast<const uint2*>(p) + i);
+      const uint2 x = reinterpret_cast<const uint2*>(p)[i];
       w[2 * i] = x.x;
       w[2 * i + 1] = x.y;
     }
   } else {
 #pragma unroll
-    for (int i = 0; i < N; ++i) w[i] = __ldcg(reinterpret_cast<const uint32_t*>(p) + i);
+    for (int i = 0; i < N; ++i) w[i] = reinterpret_cast<const uint32_t*>(p)[i];
   }
 }
 
+__device__ __forceinline__ void cp_async4(void* smem, const void* gmem) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4;\n" ::"r"(smem_u32(smem)), "l"(gmem));
+}
+
+// One unit of a warp's ring.  Rows of V are padded so that the four rows that a
+// quarter of a warp reads at once lie in different banks; rows of K need that
+// at 128 bytes only, where odd rows swap their halves.
+template <int HD>
+struct SplitStage {
+  uint8_t k[kUnit][HD];
+  uint8_t v[kUnit][HD + 16];
+  float scale[4];  // of K, of V
+};
+constexpr int kSplitStages = 3;
+
+// The values that the warps and the CTAs of a cluster join ([0] holds the CTA's
+// after the join); they take the rings' place once the units are done.
 template <int HD, int NQ>
 struct SplitShared {
-  float o[kSplitWarps][NQ][HD];  // [0] holds the CTA's joined values after the join
+  union {
+    SplitStage<HD> ring[kSplitWarps][kSplitStages];
+    float o[kSplitWarps][NQ][HD];
+  };
   float m[kSplitWarps][NQ], l[kSplitWarps][NQ];
   float cm[NQ], cl[NQ];
   uint4 qa[NQ == 16 ? HD / 16 : 1][2][32];  // A operands of the 16-query form: high, low
@@ -188,41 +208,63 @@ __global__ void __launch_bounds__(kSplitThreads, NQ == 4 ? 4 : NQ == 8 ? 3 : 2) 
 
   const int32_t* table = p.rows.page_table + static_cast<int64_t>(s) * p.rows.max_blocks;
   const int64_t head_bytes = static_cast<int64_t>(page) * HD;
-  uint32_t kw[2][KS], vw[4][VW];
-  float ks, vs;
   auto page_of = [&](int i) { return i < u1 ? __ldcg(table + ((un.at(i) * kUnit) >> lg)) : 0; };
-  // A page out of range reads page 0 and hides its positions.
-  auto load_k = [&](int i, int pg) {
+  // Unit i into stage st.  A page out of range reads page 0 and hides its positions.
+  auto fetch = [&](int i, int st, int pg) {
+    SplitStage<HD>& to = sh.ring[warp][st];
     const int64_t at = static_cast<int64_t>(pg) * p.kv.n_kv + kh;
-    const uint8_t* k0 = p.kv.k_codes + at * head_bytes + ((un.at(i) * kUnit) & (page - 1)) * HD + g * HD + t * KV;
+    const int64_t off = at * head_bytes + ((un.at(i) * kUnit) & (page - 1)) * HD;
+#pragma unroll
+    for (int j = 0; j < HD / 32; ++j) {
+      const int c = lane + 32 * j, row = c / (HD / 16), col = c % (HD / 16);
+      cp_async16(&to.k[row][(HD == 128 ? col ^ ((row & 1) * 4) : col) * 16], p.kv.k_codes + off + c * 16);
+      cp_async16(&to.v[row][col * 16], p.kv.v_codes + off + c * 16);
+    }
+    if (lane < 2) cp_async4(&to.scale[lane], (lane == 0 ? p.kv.k_scales : p.kv.v_scales) + at);
+  };
+
+  const int i0 = u0 + warp;
+  uint32_t here = 0u;  // bit j: the page of the j-th unit from here is known
+  int pg_next = page_of(i0);
+  bool lost = false;
+#pragma unroll
+  for (int j = 0; j < kSplitStages - 1; ++j) {
+    const int i = i0 + j * kSplitWarps, pg = pg_next;
+    pg_next = page_of(i + kSplitWarps);
+    if (i < u1) {
+      const bool known = pg >= 0 && pg < p.kv.n_pages;
+      here |= (known ? 1u : 0u) << j;
+      fetch(i, j, known ? pg : 0);
+    }
+    cp_async_commit();
+  }
+  int st = 0;
+  for (int i = i0; i < u1; i += kSplitWarps) {
+    const int t0 = un.at(i) * kUnit;
+    cp_async_wait<kSplitStages - 2>();
+    __syncwarp();  // every lane's copies of this unit have landed; the stage of the unit before it is free
+    {
+      const int in = i + (kSplitStages - 1) * kSplitWarps, pg = pg_next;
+      pg_next = page_of(in + kSplitWarps);
+      if (in < u1) {
+        const bool known = pg >= 0 && pg < p.kv.n_pages;
+        here |= (known ? 1u : 0u) << (kSplitStages - 1);
+        fetch(in, st == 0 ? kSplitStages - 1 : st - 1, known ? pg : 0);
+      }
+      cp_async_commit();
+    }
+    const SplitStage<HD>& un_st = sh.ring[warp][st];
+    st = st + 1 == kSplitStages ? 0 : st + 1;
+    const bool seen_here = (here & 1u) != 0u;
+    here >>= 1;
+    lost |= !seen_here;
+    const float k_scale = un_st.scale[0], v_scale = un_st.scale[1];
+    uint32_t kw[2][KS], vw[4][VW];
 #pragma unroll
     for (int j = 0; j < 2; ++j)
 #pragma unroll
-      for (int c = 0; c < KN; ++c) load_words<KW>(k0 + j * 8 * HD + c * 4 * KV, &kw[j][c * KW]);
-    ks = __ldcg(p.kv.k_scales + at);
-    vs = __ldcg(p.kv.v_scales + at);
-  };
-  auto load_v = [&](int i, int pg) {
-    const int64_t at = static_cast<int64_t>(pg) * p.kv.n_kv + kh;
-    const uint8_t* v0 = p.kv.v_codes + at * head_bytes + ((un.at(i) * kUnit) & (page - 1)) * HD + 2 * t * HD + g * VW * 4;
-#pragma unroll
-    for (int j = 0; j < 4; ++j) load_words<VW>(v0 + ((j & 1) + (j >> 1) * 8) * HD, vw[j]);
-  };
-  auto known = [&](int pg) { return pg >= 0 && pg < p.kv.n_pages; };
-
-  int i = u0 + warp;
-  int pg = page_of(i);
-  bool here = known(pg), lost = false;
-  if (i < u1) {
-    load_k(i, here ? pg : 0);
-    load_v(i, here ? pg : 0);
-  }
-  int pg_next = page_of(i + kSplitWarps);
-  for (; i < u1; i += kSplitWarps) {
-    const int t0 = un.at(i) * kUnit;
-    const bool seen_here = here;
-    lost |= !here;
-    const float k_scale = ks, v_scale = vs;
+      for (int c = 0; c < KN; ++c)
+        load_words<KW>(&un_st.k[8 * j + g][(HD == 128 ? c ^ (g & 1) : c) * 4 * KV + t * KV], &kw[j][c * KW]);
     float c[2][4];  // two chains of products: of even and odd k-steps (4 queries), of positions 0-7 and 8-15 (others)
 #pragma unroll
     for (int j = 0; j < 2; ++j) c[j][0] = c[j][1] = c[j][2] = c[j][3] = 0.f;
@@ -242,12 +284,6 @@ __global__ void __launch_bounds__(kSplitThreads, NQ == 4 ? 4 : NQ == 8 ? 3 : 2) 
         mma_f16(c[1], lo.x, lo.y, lo.z, lo.w, b0, b1);
       }
     }
-    const bool more = i + kSplitWarps < u1;
-    here = known(pg_next);
-    const int pg_load = here ? pg_next : 0;
-    if (more) load_k(i + kSplitWarps, pg_load);
-    pg_next = page_of(i + 2 * kSplitWarps);
-
     // Scores of this lane's queries: at positions t0 + g, t0 + g + 8 (4 queries), t0 + 8 j + 2 t + e (others).
     const bool plain = seen_here && t0 + kUnit - 1 <= first_pos &&
                        (p.window == 0 || t0 > last_pos - p.window || t0 + kUnit <= p.n_sink);  // all of them see all
@@ -331,6 +367,8 @@ __global__ void __launch_bounds__(kSplitThreads, NQ == 4 ? 4 : NQ == 8 ? 3 : 2) 
       split2(w[0], w[1], hi[k][0], lo[k][0]);
       split2(w[2], w[3], hi[k][1], lo[k][1]);
     }
+#pragma unroll
+    for (int j = 0; j < 4; ++j) load_words<VW>(&un_st.v[2 * t + (j & 1) + (j >> 1) * 8][g * VW * 4], vw[j]);
     const uint32_t b0 = g & 1 ? lo[0][0] : hi[0][0], b1 = g & 1 ? lo[0][1] : hi[0][1];  // 4 queries
 #pragma unroll
     for (int w = 0; w < VW; ++w) {
@@ -354,11 +392,12 @@ __global__ void __launch_bounds__(kSplitThreads, NQ == 4 ? 4 : NQ == 8 ? 3 : 2) 
         }
       }
     }
-    if (more) load_v(i + kSplitWarps, pg_load);
   }
   if (lost && lane == 0) paged_error(p.rows);
 
   // This warp's values in their own units, then the CTA's and the cluster's.
+  cp_async_wait<0>();
+  __syncthreads();
   const float unit = pow2i(max(eref, -126));
 #pragma unroll
   for (int k = 0; k < QT; ++k) {
@@ -425,8 +464,10 @@ __global__ void __launch_bounds__(kSplitThreads, NQ == 4 ? 4 : NQ == 8 ? 3 : 2) 
 template <int HD, int NQ>
 int launch_split(const PagedAttnArgs& p, int groups, int ranks, cudaStream_t s) {
   static SmemLimit configured;
+  static WideCluster wide;
   const size_t smem = sizeof(SplitShared<HD, NQ>);
   if (!ensure_smem(paged_split_kernel<HD, NQ>, smem, configured)) return NH_E_CUDA;
+  if (ranks > 8 && !ensure_wide_cluster(paged_split_kernel<HD, NQ>, wide)) return NH_E_CUDA;
   return launch_cluster(paged_split_kernel<HD, NQ>, dim3(ranks, p.kv.n_kv * groups, p.rows.n_seq), dim3(kSplitThreads),
                         ranks, smem, s, p);
 }
@@ -439,7 +480,7 @@ int launch_split_hd(const PagedAttnArgs& p, cudaStream_t s) {
   const int64_t items = static_cast<int64_t>(p.rows.n_seq) * p.kv.n_kv * groups;
   const int64_t units = static_cast<int64_t>(p.rows.max_blocks) * p.kv.page / kUnit;
   int ranks = 1;
-  while (ranks < 8 && items * ranks < 4 * device_sm_count() && units > 2 * kSplitWarps * ranks) ranks *= 2;
+  while (ranks < 16 && items * ranks < 4 * device_sm_count() && units > 2 * kSplitWarps * ranks) ranks *= 2;
   return nq == 4   ? launch_split<HD, 4>(p, groups, ranks, s)
          : nq == 8 ? launch_split<HD, 8>(p, groups, ranks, s)
                    : launch_split<HD, 16>(p, groups, ranks, s);

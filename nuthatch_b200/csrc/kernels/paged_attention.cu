@@ -19,6 +19,8 @@
 //   conversion shared by twice the queries.
 #include <cooperative_groups.h>
 
+#include <cstddef>
+
 #include "paged_attention.cuh"
 
 namespace cg = cooperative_groups;
@@ -27,9 +29,11 @@ namespace nh {
 
 namespace {
 
-constexpr int kSplitWarps = 4;
-constexpr int kSplitThreads = kSplitWarps * 32;
 constexpr int kUnit = 16;  // positions of one warp step
+// Warps of a CTA: sixteen to an SM either way by their registers, in fewer and larger CTAs for four queries (one long
+// sequence 158 -> 135 us, the decode batch 134 -> 127 us against four warps a CTA).
+template <int NQ>
+constexpr int kWarpsOf = NQ == 4 ? 8 : 4;
 
 __device__ __forceinline__ void mma_f16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
                                         uint32_t b1) {
@@ -65,8 +69,11 @@ __device__ __forceinline__ void load_words(const uint8_t* p, uint32_t* w) {
   }
 }
 
-__device__ __forceinline__ void cp_async4(void* smem, const void* gmem) {
-  asm volatile("cp.async.ca.shared.global [%0], [%1], 4;\n" ::"r"(smem_u32(smem)), "l"(gmem));
+__device__ __forceinline__ void copy16(uint32_t smem, const void* gmem) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;\n" ::"r"(smem), "l"(gmem) : "memory");
+}
+__device__ __forceinline__ void copy4(uint32_t smem, const void* gmem) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4;\n" ::"r"(smem), "l"(gmem) : "memory");
 }
 
 // One unit of a warp's ring.  Rows of V are padded so that the four rows that a
@@ -84,6 +91,7 @@ constexpr int kSplitStages = 3;
 // after the join); they take the rings' place once the units are done.
 template <int HD, int NQ>
 struct SplitShared {
+  static constexpr int kSplitWarps = kWarpsOf<NQ>;
   union {
     SplitStage<HD> ring[kSplitWarps][kSplitStages];
     float o[kSplitWarps][NQ][HD];
@@ -100,7 +108,8 @@ struct Units {
 };
 
 template <int HD, int NQ>
-__global__ void __launch_bounds__(kSplitThreads, NQ == 4 ? 4 : NQ == 8 ? 3 : 2) paged_split_kernel(const PagedAttnArgs p) {
+__global__ void __launch_bounds__(kWarpsOf<NQ> * 32, NQ == 8 ? 3 : 2) paged_split_kernel(const PagedAttnArgs p) {
+  constexpr int kSplitWarps = kWarpsOf<NQ>, kSplitThreads = kSplitWarps * 32;
   constexpr int KS = HD / 16;                    // k-steps of the score product
   constexpr int KV = HD % 64 == 0 ? 16 : 8;      // contiguous bytes of K a lane loads at once
   constexpr int KW = KV / 4, KN = HD / (4 * KV);  // words of such a piece, pieces a row
@@ -133,6 +142,69 @@ __global__ void __launch_bounds__(kSplitThreads, NQ == 4 ? 4 : NQ == 8 ? 3 : 2) 
   un.n = un.n_sink + last_pos / kUnit + 1 - un.lo;
   const int u0 = static_cast<int>(static_cast<int64_t>(un.n) * rank / nrank);
   const int u1 = static_cast<int>(static_cast<int64_t>(un.n) * (rank + 1) / nrank);
+
+  const int32_t* table = p.rows.page_table + static_cast<int64_t>(s) * p.rows.max_blocks;
+  // Copies of 16 bytes: lane l takes chunks l, l + 32, ... of a unit's 16 rows, constant steps apart in both memories.
+  constexpr unsigned kChunks = HD / 16;  // chunks of a row
+  const unsigned c_row = static_cast<unsigned>(lane) / kChunks, c_col = static_cast<unsigned>(lane) % kChunks;
+  const uint32_t page_bytes = static_cast<uint32_t>(p.kv.n_kv) * static_cast<uint32_t>(page * HD);  // below 2^30
+  const uint8_t* const k_lane = p.kv.k_codes + static_cast<uint32_t>(kh * page * HD + lane * 16);
+  const uint8_t* const v_lane = p.kv.v_codes + static_cast<uint32_t>(kh * page * HD + lane * 16);
+  const float* const s_lane = (lane == 0 ? p.kv.k_scales : p.kv.v_scales) + kh;
+  const uint32_t ring = smem_u32(&sh.ring[warp][0]);
+  const uint32_t k_to = ring + static_cast<uint32_t>(offsetof(SplitStage<HD>, k)) + c_row * HD +
+                        (HD == 128 ? c_col ^ ((c_row & 1u) * 4u) : c_col) * 16u;
+  const uint32_t v_to = ring + static_cast<uint32_t>(offsetof(SplitStage<HD>, v)) + c_row * (HD + 16) + c_col * 16u;
+  const uint32_t s_to = ring + static_cast<uint32_t>(offsetof(SplitStage<HD>, scale)) + lane * 4u;
+  // Unit i into stage st.  A page out of range reads page 0 and hides its positions.
+  auto fetch = [&](int i, int st, int pg) {
+    const uint64_t off = static_cast<uint64_t>(static_cast<uint32_t>(pg)) * page_bytes +
+                         static_cast<uint32_t>(((un.at(i) * kUnit) & (page - 1)) * HD);
+    const uint32_t to = static_cast<uint32_t>(st) * static_cast<uint32_t>(sizeof(SplitStage<HD>));
+#pragma unroll
+    for (unsigned j = 0; j < HD / 32; ++j) {
+      if constexpr (32 % kChunks == 0) {
+        constexpr unsigned kRows = 32 / kChunks;  // an even number wherever odd rows swap halves
+        copy16(k_to + to + j * kRows * HD, k_lane + off + j * 512);
+        copy16(v_to + to + j * kRows * (HD + 16), v_lane + off + j * 512);
+      } else {
+        const unsigned c = static_cast<unsigned>(lane) + 32 * j, row = c / kChunks, col = c % kChunks;
+        copy16(k_to + to + (row - c_row) * HD + (col - c_col) * 16, k_lane + off + j * 512);
+        copy16(v_to + to + (row - c_row) * (HD + 16) + (col - c_col) * 16, v_lane + off + j * 512);
+      }
+    }
+    if (lane < 2) copy4(s_to + to, s_lane + static_cast<uint64_t>(static_cast<uint32_t>(pg)) * static_cast<uint32_t>(p.kv.n_kv));
+  };
+
+  // The pages of this warp's units, 32 ahead of the fetches: lane l holds that of unit i0 + (f0 + l) * kSplitWarps, or
+  // -1 where there is none.
+  const int i0 = u0 + warp;
+  auto page_ids = [&](int f0) {
+    const int i = i0 + (f0 + lane) * kSplitWarps;
+    int pg = -1;
+    if (i < u1) {
+      pg = __ldcg(table + ((un.at(i) * kUnit) >> lg));
+      if (pg >= p.kv.n_pages) pg = -1;
+    }
+    return pg;
+  };
+  int ids = page_ids(0), ids_next = page_ids(32), fetched = 0;
+  uint32_t here = 0u;  // bit j: the page of the j-th unit from here is known
+  bool lost = false;
+  auto fetch_next = [&](int i, int st, int bit) {
+    if (i < u1) {
+      const int pg = __shfl_sync(0xffffffffu, ids, fetched & 31);
+      here |= (pg >= 0 ? 1u : 0u) << bit;
+      fetch(i, st, max(pg, 0));
+      if ((++fetched & 31) == 0) {
+        ids = ids_next;
+        ids_next = page_ids(fetched + 32);
+      }
+    }
+    cp_async_commit();
+  };
+#pragma unroll
+  for (int j = 0; j < kSplitStages - 1; ++j) fetch_next(i0 + j * kSplitWarps, j, j);
 
   // The query's operand: word w of lane t holds dimensions dim(w) .. dim(w)+3.
   auto dim = [&](int w) { return (w / KW) * (4 * KV) + t * KV + (w % KW) * 4; };
@@ -206,53 +278,12 @@ __global__ void __launch_bounds__(kSplitThreads, NQ == 4 ? 4 : NQ == 8 ? 3 : 2) 
   }
   int eref = -200;  // the accumulators are in units of 2^(eref - kWeightShift)
 
-  const int32_t* table = p.rows.page_table + static_cast<int64_t>(s) * p.rows.max_blocks;
-  const int64_t head_bytes = static_cast<int64_t>(page) * HD;
-  auto page_of = [&](int i) { return i < u1 ? __ldcg(table + ((un.at(i) * kUnit) >> lg)) : 0; };
-  // Unit i into stage st.  A page out of range reads page 0 and hides its positions.
-  auto fetch = [&](int i, int st, int pg) {
-    SplitStage<HD>& to = sh.ring[warp][st];
-    const int64_t at = static_cast<int64_t>(pg) * p.kv.n_kv + kh;
-    const int64_t off = at * head_bytes + ((un.at(i) * kUnit) & (page - 1)) * HD;
-#pragma unroll
-    for (int j = 0; j < HD / 32; ++j) {
-      const int c = lane + 32 * j, row = c / (HD / 16), col = c % (HD / 16);
-      cp_async16(&to.k[row][(HD == 128 ? col ^ ((row & 1) * 4) : col) * 16], p.kv.k_codes + off + c * 16);
-      cp_async16(&to.v[row][col * 16], p.kv.v_codes + off + c * 16);
-    }
-    if (lane < 2) cp_async4(&to.scale[lane], (lane == 0 ? p.kv.k_scales : p.kv.v_scales) + at);
-  };
-
-  const int i0 = u0 + warp;
-  uint32_t here = 0u;  // bit j: the page of the j-th unit from here is known
-  int pg_next = page_of(i0);
-  bool lost = false;
-#pragma unroll
-  for (int j = 0; j < kSplitStages - 1; ++j) {
-    const int i = i0 + j * kSplitWarps, pg = pg_next;
-    pg_next = page_of(i + kSplitWarps);
-    if (i < u1) {
-      const bool known = pg >= 0 && pg < p.kv.n_pages;
-      here |= (known ? 1u : 0u) << j;
-      fetch(i, j, known ? pg : 0);
-    }
-    cp_async_commit();
-  }
   int st = 0;
   for (int i = i0; i < u1; i += kSplitWarps) {
     const int t0 = un.at(i) * kUnit;
     cp_async_wait<kSplitStages - 2>();
     __syncwarp();  // every lane's copies of this unit have landed; the stage of the unit before it is free
-    {
-      const int in = i + (kSplitStages - 1) * kSplitWarps, pg = pg_next;
-      pg_next = page_of(in + kSplitWarps);
-      if (in < u1) {
-        const bool known = pg >= 0 && pg < p.kv.n_pages;
-        here |= (known ? 1u : 0u) << (kSplitStages - 1);
-        fetch(in, st == 0 ? kSplitStages - 1 : st - 1, known ? pg : 0);
-      }
-      cp_async_commit();
-    }
+    fetch_next(i + (kSplitStages - 1) * kSplitWarps, st == 0 ? kSplitStages - 1 : st - 1, kSplitStages - 1);
     const SplitStage<HD>& un_st = sh.ring[warp][st];
     st = st + 1 == kSplitStages ? 0 : st + 1;
     const bool seen_here = (here & 1u) != 0u;
@@ -468,8 +499,8 @@ int launch_split(const PagedAttnArgs& p, int groups, int ranks, cudaStream_t s) 
   const size_t smem = sizeof(SplitShared<HD, NQ>);
   if (!ensure_smem(paged_split_kernel<HD, NQ>, smem, configured)) return NH_E_CUDA;
   if (ranks > 8 && !ensure_wide_cluster(paged_split_kernel<HD, NQ>, wide)) return NH_E_CUDA;
-  return launch_cluster(paged_split_kernel<HD, NQ>, dim3(ranks, p.kv.n_kv * groups, p.rows.n_seq), dim3(kSplitThreads),
-                        ranks, smem, s, p);
+  return launch_cluster(paged_split_kernel<HD, NQ>, dim3(ranks, p.kv.n_kv * groups, p.rows.n_seq),
+                        dim3(kWarpsOf<NQ> * 32), ranks, smem, s, p);
 }
 
 template <int HD>
@@ -479,8 +510,9 @@ int launch_split_hd(const PagedAttnArgs& p, cudaStream_t s) {
   if (static_cast<int64_t>(p.kv.n_kv) * groups > 65535) return NH_E_ARG;
   const int64_t items = static_cast<int64_t>(p.rows.n_seq) * p.kv.n_kv * groups;
   const int64_t units = static_cast<int64_t>(p.rows.max_blocks) * p.kv.page / kUnit;
+  const int warps = nq == 4 ? kWarpsOf<4> : kWarpsOf<16>;
   int ranks = 1;
-  while (ranks < 16 && items * ranks < 4 * device_sm_count() && units > 2 * kSplitWarps * ranks) ranks *= 2;
+  while (ranks < 16 && items * ranks * warps < 16 * device_sm_count() && units > 2 * warps * ranks) ranks *= 2;
   return nq == 4   ? launch_split<HD, 4>(p, groups, ranks, s)
          : nq == 8 ? launch_split<HD, 8>(p, groups, ranks, s)
                    : launch_split<HD, 16>(p, groups, ranks, s);

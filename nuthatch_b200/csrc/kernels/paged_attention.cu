@@ -32,6 +32,7 @@ namespace {
 constexpr int kUnit = 16;  // positions of one warp step
 // Warps of a CTA: sixteen to an SM either way by their registers, in fewer and larger CTAs for four queries (one long
 // sequence 158 -> 135 us, the decode batch 134 -> 127 us against four warps a CTA).
+constexpr int kFewQueries = 16;
 template <int NQ>
 constexpr int kWarpsOf = NQ == 4 ? 8 : 4;
 
@@ -554,5 +555,14 @@ extern "C" int nh_paged_attention(const NhPagedKv* kv, const NhPagedRows* rows, 
   p.n_sink = n_sink;
   p.scale = kq_scale;
   p.few = INT32_MAX;
-  return launch_paged_split(p, static_cast<cudaStream_t>(stream));
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  if (static_cast<int64_t>(p.rows.max_rows) * p.group <= kFewQueries) return launch_paged_split(p, st);
+  if (p.rows.n_seq == 1) {
+    p.few = 0;
+    return launch_paged_tiles(p, st);
+  }
+  // Sequences of either kind may be in the call: each form passes over the other's.
+  p.few = kFewQueries;
+  const int split_rc = launch_paged_split(p, st);
+  return split_rc != NH_OK ? split_rc : launch_paged_tiles(p, st);
 }

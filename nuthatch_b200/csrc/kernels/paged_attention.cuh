@@ -56,5 +56,6 @@ __device__ __forceinline__ float exp2_fast(float x) {
 }
 
 int launch_paged_split(const PagedAttnArgs& p, cudaStream_t s);
+int launch_paged_tiles(const PagedAttnArgs& p, cudaStream_t s);
 
 }  // namespace nh

@@ -3,11 +3,13 @@
 //
 // A CTA takes 128 queries (rows x heads of one KV head) of one sequence and
 // walks the visible positions in tiles of 128:
-//   warps 4-7 read a tile's codes and write them as f16 operands (exact);
-//   warp 8 issues S = Qhi K + Qlo K and O += Phi V + Plo V (tcgen05.mma
+//   warps 8-11 read a tile's codes and write them as f16 operands (exact);
+//   warp 12 issues S = Qhi K + Qlo K and O += Phi V + Plo V (tcgen05.mma
 //   kind::f16, accumulators and P in tensor memory);
-//   warps 0-3 hold a row a lane: scores, running maximum and sum, weights split
-//   into two f16 parts.  The next tile's scores are formed meanwhile.
+//   warps 0-3 and 4-7 hold a row a lane and half of the tile's positions each:
+//   scores, running maximum (exchanged) and sum, weights split into two f16
+//   parts that take the scores' place.  The next tile's scores are formed
+//   meanwhile.
 // What bounds it: the two-part products make 8 hd products a score and row
 // where one f16 pass would make 4 (the price of f32 queries and weights); beside
 // them some 8 operations a score for the softmax.  Operands lie in shared
@@ -30,21 +32,26 @@ constexpr int kTileK = 128;     // positions of a step
 constexpr int kSub = 16;        // positions that certainly share a page
 constexpr int kSubs = kTileK / kSub;
 constexpr int kTileStages = 4;  // operand tiles in flight (K and V alternate)
-constexpr int kTileThreads = 288;
+constexpr int kTileThreads = 416;
+constexpr int kHalf = kTileK / 2;  // positions of a tile that one softmax warp takes
+constexpr float kLeast = 1.17549435e-38f;  // factor of the scores at least: a hidden one, -inf, stays that
+constexpr int kHidden = -1000;     // V's exponent where no position is seen
 constexpr int kChunkBytes = kTileK * 16;  // one 8-dimension chunk of an operand tile
 constexpr int kTileShift = 7;   // weights are 2^7 times [0, 2^8]
 constexpr float kGrow = 8.f;    // the maximum in use lags the true one by at most 2^8
 
-constexpr uint32_t kColS = 0, kColP = 256, kColO = 384, kTmemCols = 512;
+constexpr uint32_t kColS = 0, kColO = 256, kTmemCols = 512;
 
 template <int HD>
 struct TileShared {
   static constexpr int kOperand = HD / 8 * kChunkBytes;
   uint8_t q[2][kOperand];  // high, low parts
   uint8_t ring[kTileStages][kOperand];
-  float ks[4][kSubs], vs[4][kSubs];  // scales of a tile's 16-position parts (four tiles); vs 0: hidden
-  uint64_t full[kTileStages], empty[kTileStages], scales[4], q_full, s_full[2], p_full, pv_done, drained;
-  float m[kTileQ], l[kTileQ];
+  float ks[4][kSubs];  // scales of a tile's 16-position parts (four tiles)
+  int ve[4][kSubs];    // exponents of V's, or kHidden
+  float top[2][2][kTileQ];  // the halves' maxima of a row (two tiles)
+  uint64_t full[kTileStages], empty[kTileStages], scales[4], q_full, s_full[2], p_full, pv_done, drained, maxima[4];
+  float m[kTileQ], l[2][kTileQ], b[2][kTileQ];
   uint32_t tmem;
   int failed;
 };
@@ -105,6 +112,21 @@ __device__ __forceinline__ void tc_st32(uint32_t addr, const uint32_t* v) {
       NH_W8(v, 8), NH_W8(v, 16), NH_W8(v, 24), "r"(addr)
       : "memory");
 }
+__device__ __forceinline__ void tc_ld16(uint32_t addr, uint32_t* v) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];\n"
+      : NH_R8(v, 0), NH_R8(v, 8)
+      : "r"(addr)
+      : "memory");
+}
+__device__ __forceinline__ void tc_st16(uint32_t addr, const uint32_t* v) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%16], {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15};\n" ::NH_W8(
+          v, 0),
+      NH_W8(v, 8), "r"(addr)
+      : "memory");
+}
+__device__ __forceinline__ void tc_loaded16(uint32_t* v) { asm volatile("" : NH_RW8(v, 0), NH_RW8(v, 8)); }
 __device__ __forceinline__ void tc_loaded(uint32_t* v) {
   asm volatile("" : NH_RW8(v, 0), NH_RW8(v, 8), NH_RW8(v, 16), NH_RW8(v, 24));
 }
@@ -187,16 +209,17 @@ __global__ void __launch_bounds__(kTileThreads, 1) paged_tile_kernel(const Paged
       mbar_init(&sh.empty[i], 1);
     }
     for (int i = 0; i < 4; ++i) mbar_init(&sh.scales[i], 4);
-    mbar_init(&sh.q_full, kTileQ);
+    for (int i = 0; i < 4; ++i) mbar_init(&sh.maxima[i], 2);
+    mbar_init(&sh.q_full, 8);
     mbar_init(&sh.s_full[0], 1);
     mbar_init(&sh.s_full[1], 1);
-    mbar_init(&sh.p_full, kTileQ);
+    mbar_init(&sh.p_full, 8);
     mbar_init(&sh.pv_done, 1);
     mbar_init(&sh.drained, 1);
     sh.failed = 0;
     fence_barrier_init();
   }
-  if (warp == 8) {
+  if (warp == 12) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;\n" ::"r"(smem_u32(&sh.tmem)),
                  "r"(kTmemCols)
                  : "memory");
@@ -211,9 +234,9 @@ __global__ void __launch_bounds__(kTileThreads, 1) paged_tile_kernel(const Paged
   int eref = -200;                                    // O is in units of 2^(eref - kTileShift)
   bool ok = true, lost = false;
 
-  if (warp >= 4 && warp < 8) {
+  if (warp >= 8 && warp < 12) {
     // ---------------------------------------------------------------- codes to operands
-    const int w = warp - 4, r = lane & 7, c = lane >> 3;
+    const int w = warp - 8, r = lane & 7, c = lane >> 3;
     const int32_t* table = p.rows.page_table + static_cast<int64_t>(s) * p.rows.max_blocks;
     const uint64_t page_bytes = static_cast<uint64_t>(p.kv.n_kv) * static_cast<uint64_t>(page * HD);
     const uint64_t head_off = static_cast<uint64_t>(kh) * static_cast<uint64_t>(page * HD);
@@ -266,11 +289,12 @@ __global__ void __launch_bounds__(kTileThreads, 1) paged_tile_kernel(const Paged
     for (int j = 0; j < n && ok; ++j) {
       ids_of(j + 1, id_next);
       lost |= id[0] == -2 || id[1] == -2;
-      float ks = 1.f, vs = 0.f;  // vs 0: hidden
+      float ks = 1.f;
+      int ve = kHidden;
       const int mine = lane == 0 ? id[0] : id[1];
       if (lane < 2 && mine >= 0) {
         ks = __ldcg(p.kv.k_scales + static_cast<int64_t>(mine) * p.kv.n_kv + kh);
-        vs = __ldcg(p.kv.v_scales + static_cast<int64_t>(mine) * p.kv.n_kv + kh);
+        ve = exponent_of(__ldcg(p.kv.v_scales + static_cast<int64_t>(mine) * p.kv.n_kv + kh));
       }
       load(p.kv.v_codes, j, id, rv);
       ok = put(2 * j, rk);
@@ -278,7 +302,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) paged_tile_kernel(const Paged
       if (ok) {
         if (lane < 2) {
           sh.ks[j & 3][w * 2 + lane] = ks;
-          sh.vs[j & 3][w * 2 + lane] = vs;
+          sh.ve[j & 3][w * 2 + lane] = ve;
         }
         __syncwarp();
         if (lane == 0) mbar_arrive(&sh.scales[j & 3]);
@@ -288,7 +312,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) paged_tile_kernel(const Paged
       id[0] = id_next[0];
       id[1] = id_next[1];
     }
-  } else if (warp == 8) {
+  } else if (warp == 12) {
     // ---------------------------------------------------------------- products
     if (lane == 0 && n > 0) {
       const uint32_t ring = smem_u32(sh.ring[0]), qh = smem_u32(sh.q[0]), ql = smem_u32(sh.q[1]);
@@ -310,8 +334,9 @@ __global__ void __launch_bounds__(kTileThreads, 1) paged_tile_kernel(const Paged
       };
       ok = mbar_wait(&sh.q_full, 0) && scores(0);
       for (int j = 0; j < n && ok; ++j) {
-        // S of tile j + 1 takes the place of tile j - 1's, read before its weights were announced.
-        if (j + 1 < n) ok = scores(j + 1);
+        // S of tile j + 1 takes the place of tile j - 1's weights.
+        if (j > 0) ok = mbar_wait(&sh.pv_done, static_cast<uint32_t>(j - 1) & 1u);
+        if (ok && j + 1 < n) ok = scores(j + 1);
         const int use = 2 * j + 1, st = use % kTileStages;
         ok = ok && mbar_wait(&sh.full[st], static_cast<uint32_t>((use / kTileStages) & 1)) &&
              mbar_wait(&sh.p_full, static_cast<uint32_t>(j & 1));
@@ -322,7 +347,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) paged_tile_kernel(const Paged
         for (int part = 0; part < 2; ++part)
 #pragma unroll
           for (int k = 0; k < kTileK / 16; ++k)
-            mma_ts(tmem + kColO, tmem + kColP + part * (kTileK / 2) + k * 8, operand(vb + k * 256, 128, kChunkBytes),
+            mma_ts(tmem + kColO, tmem + kColS + (j & 1) * kTileK + (k >> 1) * 32 + part * 16 + (k & 1) * 8, operand(vb + k * 256, 128, kChunkBytes),
                    idesc(HD, true), j + part + k > 0);
         tc_commit(&sh.empty[st]);
         tc_commit(&sh.pv_done);
@@ -332,48 +357,51 @@ __global__ void __launch_bounds__(kTileThreads, 1) paged_tile_kernel(const Paged
       ok = mbar_wait(&sh.drained, 0) && ok;
     }
     __syncwarp();
-  } else if (warp < 4) {
-    // ---------------------------------------------------------------- softmax: a row a lane
-    const uint32_t lanes = static_cast<uint32_t>(warp * 32) << 16;
-    const bool row_ok = tid < nq;
-    const int qi = q0 + (row_ok ? tid : 0), pos = row_ok ? sq.p0 + qi / p.group : -1;
-    const bool idle = warp * 32 >= nq;  // no row of this warp is a query
-    float fq = 0.f, hq = 0.f;
+  } else {
+    // ---------------------------------------------------------------- softmax: a row a lane, half of the positions
+    const int half = warp >> 2, quad = warp & 3, row = quad * 32 + lane;
+    const uint32_t lanes = static_cast<uint32_t>(quad * 32) << 16;
+    const bool row_ok = row < nq;
+    const int qi = q0 + (row_ok ? row : 0), pos = row_ok ? sq.p0 + qi / p.group : -1;
+    const bool idle = quad * 32 >= nq;  // no row of this warp is a query
+    float fq, hq;
     {
-      const float* q = p.q + (static_cast<int64_t>(sq.r0 + qi / p.group) * p.n_head + kh * p.group + qi % p.group) * HD;
-      float4 x[HD / 4];
-      float top = 0.f;
-#pragma unroll
+      const float4* q = reinterpret_cast<const float4*>(
+          p.q + (static_cast<int64_t>(sq.r0 + qi / p.group) * p.n_head + kh * p.group + qi % p.group) * HD);
+      float top = 0.f, sum = 0.f;
+#pragma unroll 8
       for (int i = 0; i < HD / 4; ++i) {
-        x[i] = row_ok ? __ldcg(reinterpret_cast<const float4*>(q) + i) : make_float4(0.f, 0.f, 0.f, 0.f);
-        top = fmaxf(top, fmaxf(fmaxf(fabsf(x[i].x), fabsf(x[i].y)), fmaxf(fabsf(x[i].z), fabsf(x[i].w))));
+        const float4 x = row_ok ? __ldcg(q + i) : make_float4(0.f, 0.f, 0.f, 0.f);
+        top = fmaxf(top, fmaxf(fmaxf(fabsf(x.x), fabsf(x.y)), fmaxf(fabsf(x.z), fabsf(x.w))));
+        sum += (x.x + x.y) + (x.z + x.w);
       }
       // The largest magnitude goes to [2^13, 2^14); a negative factor of the scores changes the query's sign.
       const int e = min(max(exponent_of(top), -100), 126);
       const float up = p.scale < 0.f ? -pow2i(13 - e) : pow2i(13 - e);
-      float sum = 0.f;
-#pragma unroll
-      for (int i = 0; i < HD / 8; ++i) {
+#pragma unroll 4
+      for (int i = half * (HD / 16); i < (half + 1) * (HD / 16); ++i) {
+        const float4 z = make_float4(0.f, 0.f, 0.f, 0.f);
+        const float4 a = row_ok ? __ldcg(q + 2 * i) : z, b = row_ok ? __ldcg(q + 2 * i + 1) : z;
         uint4 h, l;
-        const float4 a = x[2 * i], b = x[2 * i + 1];
         split2(a.x * up, a.y * up, h.x, l.x);
         split2(a.z * up, a.w * up, h.y, l.y);
         split2(b.x * up, b.y * up, h.z, l.z);
         split2(b.z * up, b.w * up, h.w, l.w);
-        sum += ((a.x * up + a.y * up) + (a.z * up + a.w * up)) + ((b.x * up + b.y * up) + (b.z * up + b.w * up));
-        *reinterpret_cast<uint4*>(sh.q[0] + i * kChunkBytes + tid * 16) = h;
-        *reinterpret_cast<uint4*>(sh.q[1] + i * kChunkBytes + tid * 16) = l;
+        *reinterpret_cast<uint4*>(sh.q[0] + i * kChunkBytes + row * 16) = h;
+        *reinterpret_cast<uint4*>(sh.q[1] + i * kChunkBytes + row * 16) = l;
       }
-      hq = 0.5f * sum;
+      hq = 0.5f * up * sum;
       fq = fabsf(p.scale) * kLog2e * pow2i(e - 13);
       fence_async_smem();
-      mbar_arrive(&sh.q_full);
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&sh.q_full);
     }
     for (int j = 0; j < n && ok; ++j) {
       if (idle) {
         // In step with the others: the phase before must be over.
         ok = j == 0 || mbar_wait(&sh.pv_done, static_cast<uint32_t>(j - 1) & 1u);
-        mbar_arrive(&sh.p_full);
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&sh.p_full);
         continue;
       }
       ok = mbar_wait(&sh.scales[j & 3], static_cast<uint32_t>(j >> 2) & 1u) &&
@@ -383,47 +411,55 @@ __global__ void __launch_bounds__(kTileThreads, 1) paged_tile_kernel(const Paged
         break;
       }
       tc_after();
-      uint32_t u[kTileK];
-#pragma unroll
-      for (int i = 0; i < kTileK / 32; ++i) tc_ld32(tmem + kColS + (j & 1) * kTileK + lanes + i * 32, u + i * 32);
+      const uint32_t scol = tmem + kColS + (j & 1) * kTileK + lanes + half * kHalf;
+      uint32_t u[kHalf];
+      tc_ld32(scol, u);
+      tc_ld32(scol + 32, u + 32);
       const int t0 = tile_pos(j);
-      float ks[kSubs], vs[kSubs];
-      bool all = true;
-      int ev = -200;
-#pragma unroll
-      for (int b = 0; b < kSubs; ++b) {
-        ks[b] = sh.ks[j & 3][b];
-        vs[b] = sh.vs[j & 3][b];
-        all &= vs[b] != 0.f;
-        if (vs[b] != 0.f) ev = max(ev, exponent_of(vs[b]));
-      }
+      // Scales: K's of this half's four parts, V's exponents of these and of the others.
+      const float4 k4 = *reinterpret_cast<const float4*>(&sh.ks[j & 3][half * 4]);
+      const int4 v4 = *reinterpret_cast<const int4*>(&sh.ve[j & 3][half * 4]);
+      const int4 w4 = *reinterpret_cast<const int4*>(&sh.ve[j & 3][(half ^ 1) * 4]);
+      const float ks[4] = {k4.x, k4.y, k4.z, k4.w};
+      const int ve[4] = {v4.x, v4.y, v4.z, v4.w};
+      const int low_e = min(min(min(v4.x, v4.y), min(v4.z, v4.w)), min(min(w4.x, w4.y), min(w4.z, w4.w)));
+      const int ev = max(max(max(v4.x, v4.y), max(v4.z, v4.w)), max(max(w4.x, w4.y), max(w4.z, w4.w)));
       tc_wait_ld();
-#pragma unroll
-      for (int i = 0; i < kTileK / 32; ++i) tc_loaded(u + i * 32);
+      tc_loaded(u);
+      tc_loaded(u + 32);
       float* x = reinterpret_cast<float*>(u);
-      const bool plain = all && t0 + kTileK - 1 <= first_pos &&
+      const bool plain = low_e != kHidden && t0 + kTileK - 1 <= first_pos &&
                          (p.window == 0 || t0 > last_pos - p.window || t0 + kTileK <= p.n_sink);
       if (!plain) {
-        const int hi = pos - t0;                                                       // columns above it are hidden,
-        const int low = p.window > 0 ? pos - p.window - t0 : -1, sk = p.n_sink - t0;  // up to `low` unless below `sk`
+        const int h0 = t0 + half * kHalf;
+        const int hi = pos - h0;                                                       // columns above it are hidden,
+        const int low = p.window > 0 ? pos - p.window - h0 : -1, sk = p.n_sink - h0;  // up to `low` unless below `sk`
 #pragma unroll
-        for (int i = 0; i < kTileK; ++i)
-          if (i > hi || (i <= low && i >= sk) || vs[i / kSub] == 0.f) x[i] = -INFINITY;
+        for (int i = 0; i < kHalf; ++i)
+          if (i > hi || (i <= low && i >= sk) || ve[i / kSub] == kHidden) x[i] = -INFINITY;
       }
       float top = -INFINITY;
 #pragma unroll
-      for (int b = 0; b < kSubs; ++b) {
+      for (int b = 0; b < 4; ++b) {
         float t = x[b * kSub];
 #pragma unroll
         for (int i = 1; i < kSub; ++i) t = fmaxf(t, x[b * kSub + i]);
-        top = fmaxf(top, t == -INFINITY ? t : (t + hq) * (fq * ks[b]));
+        top = fmaxf(top, (t + hq) * fmaxf(fq * ks[b], kLeast));
       }
+      sh.top[j & 1][half][row] = top;
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&sh.maxima[quad]);
+      ok = mbar_wait(&sh.maxima[quad], static_cast<uint32_t>(j) & 1u);
+      if (__any_sync(0xffffffffu, !ok)) {
+        ok = false;
+        break;
+      }
+      top = fmaxf(top, sh.top[j & 1][half ^ 1][row]);
       // The maximum in use follows the true one only when that is 2^8 above it; O follows then, and when V's scale grows.
       const bool grow = top > (row_m == -INFINITY ? row_m : row_m + kGrow);
-      float alpha = 1.f;
-      const int en = max(eref, ev);
-      const bool rescale = __any_sync(0xffffffffu, grow) || en > eref;
-      if (rescale) {
+      if (__any_sync(0xffffffffu, grow) || ev > eref) {
+        const int en = max(eref, ev);
+        float alpha = 1.f;
         if (grow) {
           alpha = row_m == -INFINITY ? 0.f : exp2_fast(row_m - top);
           row_m = top;
@@ -432,56 +468,66 @@ __global__ void __launch_bounds__(kTileThreads, 1) paged_tile_kernel(const Paged
         alpha *= pow2i(max(eref - en, -200));
         row_b *= alpha;
         eref = en;
+        if (j > 0) {
+          ok = mbar_wait(&sh.pv_done, static_cast<uint32_t>(j - 1) & 1u);
+          if (__any_sync(0xffffffffu, !ok)) {
+            ok = false;
+            break;
+          }
+          tc_after();
+#pragma unroll
+          for (int i = half * (HD / 32); i < (half + 1) * (HD / 32); ++i) {
+            uint32_t o[16];
+            tc_ld16(tmem + kColO + lanes + i * 16, o);
+            tc_wait_ld();
+            tc_loaded16(o);
+#pragma unroll
+            for (int k = 0; k < 16; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * alpha);
+            tc_st16(tmem + kColO + lanes + i * 16, o);
+          }
+        }
       }
       const float base = row_m == -INFINITY ? 0.f : row_m;
-      // Weights, in pairs as high and low f16 parts: columns 0-63 of P hold the high ones, 64-127 the low ones.
-      uint32_t lo_part[kTileK / 2];
+      // Weights, in pairs as high and low f16 parts: of every 32 columns the first 16 hold the high ones.
 #pragma unroll
-      for (int b = 0; b < kSubs; ++b) {
-        const int eb = vs[b] == 0.f ? 0 : exponent_of(vs[b]) - eref + kTileShift;
-        const bool tiny = eb < -60;  // against the largest scale: the weight counts for the sum alone
-        const float a = fq * ks[b], off = hq * a - (tiny ? base : base - static_cast<float>(eb));
-        float sum = 0.f;
+      for (int c = 0; c < 2; ++c) {
+        uint32_t w[32];
 #pragma unroll
-        for (int i = 0; i < kSub / 2; ++i) {
-          const int k = b * kSub + 2 * i;
-          const float w0 = exp2_fast(fmaf(x[k], a, off)), w1 = exp2_fast(fmaf(x[k + 1], a, off));
-          sum += w0 + w1;
-          uint32_t h, l;
-          split2(w0, w1, h, l);
-          u[k / 2] = tiny ? 0u : h;
-          lo_part[k / 2] = tiny ? 0u : l;
+        for (int d = 0; d < 2; ++d) {
+          const int b = 2 * c + d, eb = ve[b] - eref + kTileShift;
+          const float a = fmaxf(fq * ks[b], kLeast);
+          float off = hq * a - base;
+          if (eb < -60) {
+            // Hidden, or a scale 2^60 below the largest: the weights count for the sum alone.
+            float sum = 0.f;
+#pragma unroll
+            for (int i = 0; i < kSub; ++i) sum += exp2_fast(fmaf(x[b * kSub + i], a, off));
+            row_l += sum;
+            off = -INFINITY;
+          } else {
+            off += static_cast<float>(eb);
+          }
+          float sum = 0.f;
+#pragma unroll
+          for (int i = 0; i < kSub / 2; ++i) {
+            const int k = b * kSub + 2 * i;
+            const float w0 = exp2_fast(fmaf(x[k], a, off)), w1 = exp2_fast(fmaf(x[k + 1], a, off));
+            sum += w0 + w1;
+            split2(w0, w1, w[d * 8 + i], w[16 + d * 8 + i]);
+          }
+          row_l += sum * pow2i(min(-eb, 60));
+          row_b += sum;
         }
-        row_l += tiny ? sum : sum * pow2i(-eb);
-        row_b += tiny ? 0.f : sum;
+        tc_st32(scol + c * 32, w);
       }
-      if (j > 0) ok = mbar_wait(&sh.pv_done, static_cast<uint32_t>(j - 1) & 1u);
-      if (__any_sync(0xffffffffu, !ok)) {
-        ok = false;
-        break;
-      }
-      tc_after();
-      if (rescale && j > 0) {
-#pragma unroll
-        for (int i = 0; i < HD / 32; ++i) {
-          uint32_t o[32];
-          tc_ld32(tmem + kColO + lanes + i * 32, o);
-          tc_wait_ld();
-          tc_loaded(o);
-#pragma unroll
-          for (int k = 0; k < 32; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * alpha);
-          tc_st32(tmem + kColO + lanes + i * 32, o);
-        }
-      }
-      tc_st32(tmem + kColP + lanes, u);
-      tc_st32(tmem + kColP + lanes + 32, u + 32);
-      tc_st32(tmem + kColP + lanes + 64, lo_part);
-      tc_st32(tmem + kColP + lanes + 96, lo_part + 32);
       tc_wait_st();
       tc_before();
-      mbar_arrive(&sh.p_full);
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&sh.p_full);
     }
     if (n > 0 && ok) ok = mbar_wait(&sh.pv_done, static_cast<uint32_t>(n - 1) & 1u);
+    sh.l[half][row] = row_l;
+    sh.b[half][row] = row_b;
     tc_after();
   }
   if (!ok) sh.failed = 1;
@@ -491,32 +537,31 @@ __global__ void __launch_bounds__(kTileThreads, 1) paged_tile_kernel(const Paged
   __syncthreads();
   tc_after();
   float* part = reinterpret_cast<float*>(nrank > 1 ? sh.ring[0] : nullptr);  // [kTileQ][HD]
-  if (warp < 4) {
-    const uint32_t lanes = static_cast<uint32_t>(warp * 32) << 16;
-    const int qi = q0 + tid;
+  if (warp < 8) {
+    const int half = warp >> 2, row = (warp & 3) * 32 + lane;
+    const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
+    const int qi = q0 + row;
     float* out = p.out + (static_cast<int64_t>(sq.r0 + qi / p.group) * p.n_head + kh * p.group + qi % p.group) * HD;
-    const float unit = pow2i(max(eref, -126)) ;
-    const float inv = nrank > 1 ? 1.f : row_l > 0.f ? 1.f / row_l : row_l == 0.f ? 0.f : row_l;
-    if (nrank > 1) {
-      sh.m[tid] = row_m;
-      sh.l[tid] = row_l;
-    }
+    const float l = sh.l[0][row] + sh.l[1][row], b = 0.5f * (sh.b[0][row] + sh.b[1][row]);
+    const float unit = pow2i(max(eref, -126));
+    const float inv = nrank > 1 ? 1.f : l == 0.f ? 0.f : 1.f / l;
+    if (nrank > 1 && half == 0) sh.m[row] = row_m;
 #pragma unroll
-    for (int i = 0; i < HD / 32; ++i) {
-      uint32_t o[32];
+    for (int i = half * (HD / 32); i < (half + 1) * (HD / 32); ++i) {
+      uint32_t o[16];
       if (n > 0) {
-        tc_ld32(tmem + kColO + lanes + i * 32, o);
+        tc_ld16(tmem + kColO + lanes + i * 16, o);
         tc_wait_ld();
-        tc_loaded(o);
+        tc_loaded16(o);
       }
-      float4* to = reinterpret_cast<float4*>(nrank > 1 ? part + tid * HD + i * 32 : out + i * 32);
-      if (tid < nq) {
+      float4* to = reinterpret_cast<float4*>(nrank > 1 ? part + row * HD + i * 16 : out + i * 16);
+      if (row < nq) {
 #pragma unroll
-        for (int k = 0; k < 8; ++k) {
+        for (int k = 0; k < 4; ++k) {
           float v[4];
 #pragma unroll
           for (int e = 0; e < 4; ++e)
-            v[e] = n > 0 ? (__uint_as_float(o[4 * k + e]) + 0.5f * row_b) * pow2i(-kTileShift) * unit * inv : 0.f;
+            v[e] = n > 0 ? (__uint_as_float(o[4 * k + e]) + b) * pow2i(-kTileShift) * unit * inv : 0.f;
           to[k] = make_float4(v[0], v[1], v[2], v[3]);
         }
       }
@@ -535,7 +580,8 @@ __global__ void __launch_bounds__(kTileThreads, 1) paged_tile_kernel(const Paged
         const float mr = cluster.map_shared_rank(sh.m, r)[row];
         const float a = mr == -INFINITY ? 0.f : exp2_fast(mr - top);
         const float4 y = reinterpret_cast<const float4*>(cluster.map_shared_rank(part, r))[i];
-        sum += a * cluster.map_shared_rank(sh.l, r)[row];
+        const float* lr = cluster.map_shared_rank(&sh.l[0][0], r);
+        sum += a * (lr[row] + lr[kTileQ + row]);
         v.x += a * y.x;
         v.y += a * y.y;
         v.z += a * y.z;
@@ -550,7 +596,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) paged_tile_kernel(const Paged
     __syncthreads();
   }
   if (tid == 0 && sh.failed != 0 && p.rows.err != nullptr) atomicCAS(p.rows.err, 0, NH_E_TIMEOUT);
-  if (warp == 8) {
+  if (warp == 12) {
     tc_after();
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;\n" ::"r"(tmem), "r"(kTmemCols) : "memory");
   }

@@ -3,19 +3,22 @@
 //
 // A CTA takes 128 queries (rows x heads of one KV head) of one sequence and
 // walks the visible positions in tiles of 128:
-//   warps 8-11 read a tile's codes and write them as f16 operands (exact);
-//   warp 12 issues S = Qhi K + Qlo K and O += Phi V + Plo V (tcgen05.mma
-//   kind::f16, accumulators and P in tensor memory);
+//   warps 8-11 (K) and 12-15 (V) read a tile's codes and write them as f16
+//   operands (exact);
+//   warp 16 issues S = Qhi K + Qlo K and O += Phi V + Plo V (tcgen05.mma
+//   kind::f16; accumulators, Q and P in tensor memory);
 //   warps 0-3 and 4-7 hold a row a lane and half of the tile's positions each:
 //   scores, running maximum (exchanged) and sum, weights split into two f16
-//   parts that take the scores' place.  The next tile's scores are formed
-//   meanwhile.
+//   parts that take the scores' place.
+// Two or three score tiles rotate (what the tensor memory holds), so that the
+// tensor cores form the scores ahead while weights are in the making.
 // What bounds it: the two-part products make 8 hd products a score and row
 // where one f16 pass would make 4 (the price of f32 queries and weights); beside
 // them some 8 operations a score for the softmax.  Operands lie in shared
 // memory as [8-dimension chunk][row][16 bytes], unswizzled: the same image
 // serves K (K-major) and V (MN-major), and eight lanes write 128 contiguous
-// bytes.
+// bytes.  (Unswizzled operands are read at half the shared-memory rate: with Q
+// in shared memory too, a 16-wide step of the scores took 138 cycles for 64.)
 // All waits are bounded; an expired one records NH_E_TIMEOUT.
 #include <cooperative_groups.h>
 
@@ -31,8 +34,8 @@ constexpr int kTileQ = 128;     // queries of a CTA = tensor-memory lanes
 constexpr int kTileK = 128;     // positions of a step
 constexpr int kSub = 16;        // positions that certainly share a page
 constexpr int kSubs = kTileK / kSub;
-constexpr int kTileStages = 4;  // operand tiles in flight (K and V alternate)
-constexpr int kTileThreads = 416;
+constexpr int kTileThreads = 640;
+constexpr int kSoftThreads = 256;
 constexpr int kHalf = kTileK / 2;  // positions of a tile that one softmax warp takes
 constexpr float kLeast = 1.17549435e-38f;  // factor of the scores at least: a hidden one, -inf, stays that
 constexpr int kHidden = -1000;     // V's exponent where no position is seen
@@ -40,17 +43,29 @@ constexpr int kChunkBytes = kTileK * 16;  // one 8-dimension chunk of an operand
 constexpr int kTileShift = 7;   // weights are 2^7 times [0, 2^8]
 constexpr float kGrow = 8.f;    // the maximum in use lags the true one by at most 2^8
 
-constexpr uint32_t kColS = 0, kColO = 256, kTmemCols = 512;
+constexpr uint32_t kTmemCols = 512;
+
+// Tensor-memory columns: the score tiles, O, Q (high parts, then low ones).
+template <int HD>
+struct TileTmem {
+  static constexpr int kScoreTiles = HD <= 64 ? 3 : 2;
+  static constexpr uint32_t kS = 0, kO = kScoreTiles * kTileK, kQ = kO + HD;
+  static_assert(kQ + HD <= kTmemCols, "tensor memory");
+};
 
 template <int HD>
 struct TileShared {
-  static constexpr int kOperand = HD / 8 * kChunkBytes;
-  uint8_t q[2][kOperand];  // high, low parts
-  uint8_t ring[kTileStages][kOperand];
+  static constexpr int kOperand = HD / 8 * kChunkBytes, kScoreTiles = TileTmem<HD>::kScoreTiles;
+  static constexpr int kRow = HD + 4;  // floats of a joined row, padded against bank conflicts
+  uint8_t ring[2][2][kOperand];        // K, V: two stages each
+  // Q's parts on their way to tensor memory ([row][high, low] f16); the joined values once the products are done.
+  float rows[kTileQ][kRow];
   float ks[4][kSubs];  // scales of a tile's 16-position parts (four tiles)
   int ve[4][kSubs];    // exponents of V's, or kHidden
   float top[2][2][kTileQ];  // the halves' maxima of a row (two tiles)
-  uint64_t full[kTileStages], empty[kTileStages], scales[4], q_full, s_full[2], p_full, pv_done, drained, maxima[4];
+  float fq[kTileQ], hq[kTileQ];
+  int64_t row_at[kTileQ];  // where a query's row starts in q and out
+  uint64_t full[2][2], empty[2][2], scales[4], q_full, s_full[kScoreTiles], p_full[kScoreTiles], pv_done[kScoreTiles], drained;
   float m[kTileQ], l[2][kTileQ], b[2][kTileQ];
   uint32_t tmem;
   int failed;
@@ -76,17 +91,20 @@ __device__ __forceinline__ uint64_t operand(uint32_t addr, uint32_t lead, uint32
 __host__ __device__ constexpr uint32_t idesc(int n, bool mn_major) {
   return (1u << 4) | (mn_major ? 1u << 16 : 0u) | (static_cast<uint32_t>(n >> 3) << 17) | (128u >> 4 << 24);
 }
-__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t id, bool add) {
-  asm volatile(
-      "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}\n" ::"r"(d),
-      "l"(a), "l"(b), "r"(id), "r"(add ? 1 : 0)
-      : "memory");
-}
-__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t id, bool add) {
+// D (+)= A B with A in tensor memory; a 16-wide step of B is a constant added to
+// its descriptor's low word.
+template <uint32_t kIdesc>
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t add) {
   asm volatile(
       "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}\n" ::"r"(d),
-      "r"(a), "l"(b), "r"(id), "r"(add ? 1 : 0)
+      "r"(a), "l"(b), "r"(kIdesc), "r"(add)
       : "memory");
+}
+// One lane of the warp, always the same.
+__device__ __forceinline__ bool elect_one() {
+  uint32_t is;
+  asm volatile("{\n .reg .pred p;\n elect.sync _|p, 0xffffffff;\n selp.u32 %0, 1, 0, p;\n}\n" : "=r"(is));
+  return is != 0u;
 }
 
 #define NH_R8(a, i) "=r"(a[i]), "=r"(a[i + 1]), "=r"(a[i + 2]), "=r"(a[i + 3]), "=r"(a[i + 4]), "=r"(a[i + 5]), \
@@ -136,42 +154,62 @@ __device__ __forceinline__ void tc_loaded(uint32_t* v) {
 __device__ __forceinline__ void tc_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;\n" ::: "memory"); }
 __device__ __forceinline__ void tc_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;\n" ::: "memory"); }
 
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float d;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
+// Two f32 operations in one instruction, each rounded as by itself.
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+  float2 d;
+  asm("{\n .reg .b64 x, y, z;\n mov.b64 x, {%2, %3};\n mov.b64 y, {%4, %5};\n mov.b64 z, {%6, %7};\n"
+      " fma.rn.f32x2 x, x, y, z;\n mov.b64 {%0, %1}, x;\n}\n"
+      : "=f"(d.x), "=f"(d.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+  return d;
+}
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+  float2 d;
+  asm("{\n .reg .b64 x, y;\n mov.b64 x, {%2, %3};\n mov.b64 y, {%4, %5};\n add.rn.f32x2 x, x, y;\n"
+      " mov.b64 {%0, %1}, x;\n}\n"
+      : "=f"(d.x), "=f"(d.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return d;
+}
+
 // Tiles of a sequence in this form.
-__device__ __forceinline__ int tiles_of(const PagedAttnArgs& p, int s, int64_t cap) {
-  const int64_t n_q = static_cast<int64_t>(seq_rows(p.rows, s, cap).n) * p.group;
+__device__ __forceinline__ int tiles_of(const PagedAttnArgs& p, const SeqRows& r) {
+  const int64_t n_q = static_cast<int64_t>(r.n) * p.group;
   return n_q > p.few ? static_cast<int>((n_q + kTileQ - 1) / kTileQ) : 0;
 }
 
-// The sequence and tile of `item`, later tiles (which see more positions)
-// first; false when there are not that many.  Warp-wide.
-__device__ __forceinline__ bool find_tile(const PagedAttnArgs& p, int64_t cap, int64_t item, int lane, int& seq, int& tile) {
-  int64_t total = 0;
-  for (int s0 = 0; s0 < p.rows.n_seq; s0 += 32) {
-    int n = s0 + lane < p.rows.n_seq ? tiles_of(p, s0 + lane, cap) : 0;
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) n += __shfl_xor_sync(0xffffffffu, n, o);
-    total += n;
-  }
-  if (item >= total) return false;
-  const int64_t want = total - 1 - item;
-  int64_t base = 0;
-  for (int s0 = 0; s0 < p.rows.n_seq; s0 += 32) {
-    const int mine = s0 + lane < p.rows.n_seq ? tiles_of(p, s0 + lane, cap) : 0;
-    int inc = mine;
+// The rows and tile of `item`, later tiles (which see more positions) first;
+// false when there are not that many.  Warp-wide, 32 sequences at a time, from
+// the last one on.
+__device__ __forceinline__ bool find_tile(const PagedAttnArgs& p, int64_t cap, int64_t item, int lane, int& seq, int& tile,
+                                          SeqRows& rows) {
+  for (int s0 = (p.rows.n_seq - 1) & ~31; s0 >= 0; s0 -= 32) {
+    const int s = s0 + lane;
+    SeqRows r{0, 0, 0};
+    if (s < p.rows.n_seq) r = seq_rows(p.rows, s, cap);
+    const int mine = tiles_of(p, r);
+    int inc = mine;  // tiles of this sequence and the later ones of the 32
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
-      const int up = __shfl_up_sync(0xffffffffu, inc, o);
-      if (lane >= o) inc += up;
+      const int down = __shfl_down_sync(0xffffffffu, inc, o);
+      if (lane + o < 32) inc += down;
     }
-    const int sum = __shfl_sync(0xffffffffu, inc, 31);
-    if (want < base + sum) {
-      const unsigned over = __ballot_sync(0xffffffffu, base + inc > want);
-      const int l = __ffs(over) - 1;
+    const int sum = __shfl_sync(0xffffffffu, inc, 0);
+    if (item < sum) {
+      const int l = 31 - __clz(__ballot_sync(0xffffffffu, inc > item));
       seq = s0 + l;
-      tile = static_cast<int>(want - base) - __shfl_sync(0xffffffffu, inc - mine, l);
+      tile = __shfl_sync(0xffffffffu, inc, l) - 1 - static_cast<int>(item);
+      rows.r0 = __shfl_sync(0xffffffffu, r.r0, l);
+      rows.n = __shfl_sync(0xffffffffu, r.n, l);
+      rows.p0 = __shfl_sync(0xffffffffu, r.p0, l);
       return true;
     }
-    base += sum;
+    item -= sum;
   }
   return false;
 }
@@ -185,14 +223,46 @@ __global__ void __launch_bounds__(kTileThreads, 1) paged_tile_kernel(const Paged
   const int rank = static_cast<int>(cluster.block_rank()), nrank = static_cast<int>(cluster.num_blocks());
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int page = p.kv.page, lg = p.kv.page_log2;
+  constexpr int kScoreTiles = TileTmem<HD>::kScoreTiles;
+  if (tid == 0) {
+    for (int i = 0; i < 4; ++i) {
+      mbar_init(&sh.full[i >> 1][i & 1], 4);
+      mbar_init(&sh.empty[i >> 1][i & 1], 1);
+      mbar_init(&sh.scales[i], 4);
+    }
+    mbar_init(&sh.q_full, 8);
+    for (int i = 0; i < kScoreTiles; ++i) {
+      mbar_init(&sh.s_full[i], 1);
+      mbar_init(&sh.p_full[i], 8);
+      mbar_init(&sh.pv_done[i], 1);
+    }
+    mbar_init(&sh.drained, 1);
+    sh.failed = 0;
+    fence_barrier_init();
+  }
+  if (warp == 16) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;\n" ::"r"(smem_u32(&sh.tmem)),
+                 "r"(kTmemCols)
+                 : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;\n" ::: "memory");
+  }
   pdl_wait();
   pdl_trigger();
   const int64_t cap = static_cast<int64_t>(p.rows.max_blocks) * page;
   const int64_t item = static_cast<int64_t>(blockIdx.x) / nrank;
   const int kh = static_cast<int>(item % p.kv.n_kv);
   int s = 0, qt = 0;
-  if (!find_tile(p, cap, item / p.kv.n_kv, lane, s, qt)) return;  // every CTA of the cluster alike
-  const SeqRows sq = seq_rows(p.rows, s, cap);
+  SeqRows sq{0, 0, 0};
+  const bool work = find_tile(p, cap, item / p.kv.n_kv, lane, s, qt, sq);  // every CTA of the cluster alike
+  tc_before();
+  __syncthreads();
+  tc_after();
+  const uint32_t tmem = sh.tmem;
+  if (!work) {
+    if (warp == 16)
+      asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;\n" ::"r"(tmem), "r"(kTmemCols) : "memory");
+    return;
+  }
   const int n_q = sq.n * p.group, q0 = qt * kTileQ, nq = min(kTileQ, n_q - q0);
   const int first_pos = sq.p0 + q0 / p.group, last_pos = sq.p0 + (q0 + nq - 1) / p.group;
   // Visible tiles: the sinks', then those from `lo` on; this CTA's share of them.
@@ -203,215 +273,250 @@ __global__ void __launch_bounds__(kTileThreads, 1) paged_tile_kernel(const Paged
   const int n = static_cast<int>(static_cast<int64_t>(n_all) * (rank + 1) / nrank) - j0;
   auto tile_pos = [&](int j) { return (j0 + j < n_sink ? j0 + j : j0 + j - n_sink + lo) * kTileK; };
 
-  if (tid == 0) {
-    for (int i = 0; i < kTileStages; ++i) {
-      mbar_init(&sh.full[i], 4);
-      mbar_init(&sh.empty[i], 1);
-    }
-    for (int i = 0; i < 4; ++i) mbar_init(&sh.scales[i], 4);
-    for (int i = 0; i < 4; ++i) mbar_init(&sh.maxima[i], 2);
-    mbar_init(&sh.q_full, 8);
-    mbar_init(&sh.s_full[0], 1);
-    mbar_init(&sh.s_full[1], 1);
-    mbar_init(&sh.p_full, 8);
-    mbar_init(&sh.pv_done, 1);
-    mbar_init(&sh.drained, 1);
-    sh.failed = 0;
-    fence_barrier_init();
-  }
-  if (warp == 12) {
-    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;\n" ::"r"(smem_u32(&sh.tmem)),
-                 "r"(kTmemCols)
-                 : "memory");
-    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;\n" ::: "memory");
-  }
-  tc_before();
-  __syncthreads();
-  tc_after();
-  const uint32_t tmem = sh.tmem;
-
-  float row_m = -INFINITY, row_l = 0.f, row_b = 0.f;  // a softmax lane's row: maximum in use, sum, sum in units of V
-  int eref = -200;                                    // O is in units of 2^(eref - kTileShift)
-  bool ok = true, lost = false;
-
-  if (warp >= 8 && warp < 12) {
+  // Barriers.  A wait tells a phase's parity from the next one's only, so none may run two phases ahead of a waiter: one
+  // barrier a place (score tile, operand stage), whose next phase needs what the waiter does after this one.
+  auto products_done = [&](int j) {
+    return mbar_wait(&sh.pv_done[j % kScoreTiles], static_cast<uint32_t>(j / kScoreTiles) & 1u);
+  };
+  auto all = [](bool lane_ok) { return __all_sync(0xffffffffu, lane_ok) != 0; };
+  bool ok = true;
+  if (warp >= 8 && warp < 16) {
     // ---------------------------------------------------------------- codes to operands
-    const int w = warp - 8, r = lane & 7, c = lane >> 3;
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 72;\n");
+    const int of_v = (warp - 8) >> 2, w = warp & 3, r = lane & 7, c = lane >> 3;
+    const uint8_t* codes = (of_v ? p.kv.v_codes : p.kv.k_codes) + static_cast<uint64_t>(kh) * static_cast<uint32_t>(page * HD);
+    const uint32_t page_bytes = static_cast<uint32_t>(p.kv.n_kv) * static_cast<uint32_t>(page * HD);  // at most 2^30
     const int32_t* table = p.rows.page_table + static_cast<int64_t>(s) * p.rows.max_blocks;
-    const uint64_t page_bytes = static_cast<uint64_t>(p.kv.n_kv) * static_cast<uint64_t>(page * HD);
-    const uint64_t head_off = static_cast<uint64_t>(kh) * static_cast<uint64_t>(page * HD);
-    // Pages of this warp's two 16-position parts of tile j; -1: none (past the last position), -2: out of range.
-    auto ids_of = [&](int j, int (&id)[2]) {
+    // Pages of this warp's two 16-position parts of 16 tiles: lane l has part l & 1 of tile f + (l >> 1).  -1: none (past
+    // the last position), -2: out of range.
+    auto ids_of = [&](int f) {
+      const int j = f + (lane >> 1);
+      int id = -1;
+      if (j < n) {
+        const int t = tile_pos(j) + w * 32 + (lane & 1) * kSub;
+        if (t <= last_pos) {
+          id = __ldcg(table + (t >> lg));
+          if (id < 0 || id >= p.kv.n_pages) id = -2;
+        }
+      }
+      return id;
+    };
+    // Piece i of a lane: 16 codes of row `rg` * 8 + r of the warp's 32, from column `col` * 16 on.
+    auto rg_of = [&](int i) {
+      return HD == 128 ? i >> 1 : HD == 64 ? i : HD == 32 ? 2 * i + (c >> 1) : (i * 4 + c) / kItems;
+    };
+    auto col_of = [&](int i) {
+      return HD == 128 ? (i & 1) * 4 + c : HD == 64 ? c : HD == 32 ? c & 1 : (i * 4 + c) % kItems;
+    };
+    uint4 raw[kItems];
+    int id0 = 0, id1 = 0, ids = ids_of(0), ids_next = ids_of(16);
+    float ks = 1.f, vs = 0.f;
+    bool seen = false;
+    auto load = [&](int j) {
+      id0 = __shfl_sync(0xffffffffu, ids, (j & 15) * 2);
+      id1 = __shfl_sync(0xffffffffu, ids, (j & 15) * 2 + 1);
+      if ((j & 15) == 15) {
+        ids = ids_next;
+        ids_next = ids_of(j + 17);
+      }
+      const int slot = (tile_pos(j) + w * 32 + r) & (page - 1);
+      const uint8_t* p0 = codes + static_cast<uint64_t>(static_cast<uint32_t>(max(id0, 0))) * page_bytes + slot * HD;
+      const uint8_t* p1 = codes + static_cast<uint64_t>(static_cast<uint32_t>(max(id1, 0))) * page_bytes +
+                          ((slot + kSub) & (page - 1)) * HD;
 #pragma unroll
-      for (int b = 0; b < 2; ++b) {
-        id[b] = -1;
-        if (j < n) {
-          const int t = tile_pos(j) + w * 32 + b * kSub;
-          if (t <= last_pos) {
-            const int pg = __ldcg(table + (t >> lg));
-            id[b] = pg >= 0 && pg < p.kv.n_pages ? pg : -2;
-          }
+      for (int i = 0; i < kItems; ++i) {
+        const int rg = rg_of(i);
+        raw[i] = __ldcg(reinterpret_cast<const uint4*>((rg < 2 ? p0 : p1) + (rg & 1) * 8 * HD + col_of(i) * 16));
+      }
+      if (!of_v) {
+        const int mine = lane == 0 ? id0 : id1;
+        seen = mine >= 0;
+        if (lane < 2 && seen) {
+          ks = __ldcg(p.kv.k_scales + static_cast<int64_t>(mine) * p.kv.n_kv + kh);
+          vs = __ldcg(p.kv.v_scales + static_cast<int64_t>(mine) * p.kv.n_kv + kh);
         }
       }
     };
-    auto load = [&](const uint8_t* codes, int j, const int (&id)[2], uint4 (&raw)[kItems]) {
-      const int t0 = tile_pos(j) + w * 32;
+    bool lost = false;
+    if (n > 0) load(0);
+    for (int j = 0; j < n; ++j) {
+      lost |= id0 == -2 || id1 == -2;
+      ok = all(mbar_wait(&sh.empty[of_v][j & 1], static_cast<uint32_t>((j >> 1) & 1) ^ 1u));
+      if (!ok) break;
+      uint8_t* to = sh.ring[of_v][j & 1] + (w * 32 + r) * 16;
 #pragma unroll
       for (int i = 0; i < kItems; ++i) {
-        const int it = i * 4 + c, rg = it / kItems, col = it % kItems, pg = rg < 2 ? id[0] : id[1];
-        raw[i] = pg >= 0 ? __ldcg(reinterpret_cast<const uint4*>(codes + static_cast<uint64_t>(pg) * page_bytes + head_off +
-                                                                 ((t0 + rg * 8 + r) & (page - 1)) * HD + col * 16))
-                         : make_uint4(0u, 0u, 0u, 0u);
-      }
-    };
-    auto put = [&](int use, const uint4 (&raw)[kItems]) {  // the use-th operand tile
-      const int st = use % kTileStages;
-      if (!mbar_wait(&sh.empty[st], static_cast<uint32_t>((use / kTileStages) & 1) ^ 1u)) return false;
-      uint8_t* to = sh.ring[st] + (w * 32 + r) * 16;
-#pragma unroll
-      for (int i = 0; i < kItems; ++i) {
-        const int it = i * 4 + c, rg = it / kItems, col = it % kItems;
-        uint8_t* d = to + rg * 128 + col * 2 * kChunkBytes;
+        uint8_t* d = to + rg_of(i) * 128 + col_of(i) * 2 * kChunkBytes;
         *reinterpret_cast<uint4*>(d) =
             make_uint4(codes_lo(raw[i].x), codes_hi(raw[i].x), codes_lo(raw[i].y), codes_hi(raw[i].y));
         *reinterpret_cast<uint4*>(d + kChunkBytes) =
             make_uint4(codes_lo(raw[i].z), codes_hi(raw[i].z), codes_lo(raw[i].w), codes_hi(raw[i].w));
       }
+      // The scales' place was last read for tile j - 4, whose weights were in use before K of tile j found its stage free.
+      if (!of_v && lane < 2) {
+        sh.ks[j & 3][w * 2 + lane] = seen ? ks : 1.f;
+        sh.ve[j & 3][w * 2 + lane] = seen ? exponent_of(vs) : kHidden;
+      }
       fence_async_smem();
       __syncwarp();
-      if (lane == 0) mbar_arrive(&sh.full[st]);
-      return true;
-    };
-    int id[2], id_next[2];
-    uint4 rk[kItems], rv[kItems];
-    ids_of(0, id);
-    if (n > 0) load(p.kv.k_codes, 0, id, rk);
-    for (int j = 0; j < n && ok; ++j) {
-      ids_of(j + 1, id_next);
-      lost |= id[0] == -2 || id[1] == -2;
-      float ks = 1.f;
-      int ve = kHidden;
-      const int mine = lane == 0 ? id[0] : id[1];
-      if (lane < 2 && mine >= 0) {
-        ks = __ldcg(p.kv.k_scales + static_cast<int64_t>(mine) * p.kv.n_kv + kh);
-        ve = exponent_of(__ldcg(p.kv.v_scales + static_cast<int64_t>(mine) * p.kv.n_kv + kh));
+      if (lane == 0) {
+        mbar_arrive(&sh.full[of_v][j & 1]);
+        if (!of_v) mbar_arrive(&sh.scales[j & 3]);
       }
-      load(p.kv.v_codes, j, id, rv);
-      ok = put(2 * j, rk);
-      // The scales' place was last read for tile j - 4, whose weights are in use before K of tile j finds its stage free.
-      if (ok) {
-        if (lane < 2) {
-          sh.ks[j & 3][w * 2 + lane] = ks;
-          sh.ve[j & 3][w * 2 + lane] = ve;
+      if (j + 1 < n) load(j + 1);
+    }
+    if (lost && lane == 0) paged_error(p.rows);
+    if (!ok) sh.failed = 1;
+  } else if (warp >= 16) {
+    // ---------------------------------------------------------------- products
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 48;\n");
+    if (warp == 16 && n > 0) {
+      constexpr uint32_t kOp = TileShared<HD>::kOperand;
+      constexpr uint64_t kStepK = 2 * kChunkBytes >> 4, kStepV = 256 >> 4;  // 16 dimensions of Q and K, 16 positions of V
+      const bool one = elect_one();
+      const uint64_t kd = operand(smem_u32(sh.ring[0][0]), kChunkBytes, 128);
+      const uint64_t vd = operand(smem_u32(sh.ring[1][0]), 128, kChunkBytes);
+      const uint32_t qa = tmem + TileTmem<HD>::kQ, oa = tmem + TileTmem<HD>::kO;
+      auto scores = [&](int j) {
+        if (!all(mbar_wait(&sh.full[0][j & 1], static_cast<uint32_t>(j >> 1) & 1u))) return false;
+        tc_after();
+        const uint64_t b = kd + ((j & 1) * kOp >> 4);
+        const uint32_t d = tmem + TileTmem<HD>::kS + (j % kScoreTiles) * kTileK;
+        if (one) {
+#pragma unroll
+          for (int k = 0; k < HD / 8; ++k)  // the high parts' steps, then the low ones'
+            mma_ts<idesc(kTileK, false)>(d, qa + k * 8, b + (k % (HD / 16)) * kStepK, k > 0 ? 1u : 0u);
+          tc_commit(&sh.empty[0][j & 1]);
+          tc_commit(&sh.s_full[j % kScoreTiles]);
         }
         __syncwarp();
-        if (lane == 0) mbar_arrive(&sh.scales[j & 3]);
-        if (j + 1 < n) load(p.kv.k_codes, j + 1, id_next, rk);
-        ok = put(2 * j + 1, rv);
-      }
-      id[0] = id_next[0];
-      id[1] = id_next[1];
-    }
-  } else if (warp == 12) {
-    // ---------------------------------------------------------------- products
-    if (lane == 0 && n > 0) {
-      const uint32_t ring = smem_u32(sh.ring[0]), qh = smem_u32(sh.q[0]), ql = smem_u32(sh.q[1]);
-      constexpr uint32_t kOp = TileShared<HD>::kOperand;
-      auto scores = [&](int j) {
-        const int use = 2 * j, st = use % kTileStages;
-        if (!mbar_wait(&sh.full[st], static_cast<uint32_t>((use / kTileStages) & 1))) return false;
-        tc_after();
-        const uint32_t kb = ring + st * kOp, d = tmem + kColS + (j & 1) * kTileK;
-#pragma unroll
-        for (int part = 0; part < 2; ++part)
-#pragma unroll
-          for (int k = 0; k < HD / 16; ++k)
-            mma_ss(d, operand((part == 0 ? qh : ql) + k * 2 * kChunkBytes, kChunkBytes, 128),
-                   operand(kb + k * 2 * kChunkBytes, kChunkBytes, 128), idesc(kTileK, false), part + k > 0);
-        tc_commit(&sh.empty[st]);
-        tc_commit(&sh.s_full[j & 1]);
         return true;
       };
-      ok = mbar_wait(&sh.q_full, 0) && scores(0);
+      ok = all(mbar_wait(&sh.q_full, 0)) && scores(0) && (n < 2 || scores(1));
       for (int j = 0; j < n && ok; ++j) {
-        // S of tile j + 1 takes the place of tile j - 1's weights.
-        if (j > 0) ok = mbar_wait(&sh.pv_done, static_cast<uint32_t>(j - 1) & 1u);
-        if (ok && j + 1 < n) ok = scores(j + 1);
-        const int use = 2 * j + 1, st = use % kTileStages;
-        ok = ok && mbar_wait(&sh.full[st], static_cast<uint32_t>((use / kTileStages) & 1)) &&
-             mbar_wait(&sh.p_full, static_cast<uint32_t>(j & 1));
+        ok = mbar_wait(&sh.full[1][j & 1], static_cast<uint32_t>(j >> 1) & 1u) &&
+             mbar_wait(&sh.p_full[j % kScoreTiles], static_cast<uint32_t>(j / kScoreTiles) & 1u);
+        // With three score tiles, those of j + 2 will take the place of tile j - 1's weights.
+        if (kScoreTiles == 3 && ok && j > 0) ok = products_done(j - 1);
+        ok = all(ok);
         if (!ok) break;
         tc_after();
-        const uint32_t vb = ring + st * kOp;
-#pragma unroll
-        for (int part = 0; part < 2; ++part)
+        const uint64_t b = vd + ((j & 1) * kOp >> 4);
+        const uint32_t a = tmem + TileTmem<HD>::kS + (j % kScoreTiles) * kTileK;
+        if (one) {
 #pragma unroll
           for (int k = 0; k < kTileK / 16; ++k)
-            mma_ts(tmem + kColO, tmem + kColS + (j & 1) * kTileK + (k >> 1) * 32 + part * 16 + (k & 1) * 8, operand(vb + k * 256, 128, kChunkBytes),
-                   idesc(HD, true), j + part + k > 0);
-        tc_commit(&sh.empty[st]);
-        tc_commit(&sh.pv_done);
+            mma_ts<idesc(HD, true)>(oa, a + (k >> 1) * 32 + (k & 1) * 8, b + k * kStepV, k > 0 || j > 0 ? 1u : 0u);
+#pragma unroll
+          for (int k = 0; k < kTileK / 16; ++k)
+            mma_ts<idesc(HD, true)>(oa, a + (k >> 1) * 32 + 16 + (k & 1) * 8, b + k * kStepV, 1u);
+          tc_commit(&sh.empty[1][j & 1]);
+          tc_commit(&sh.pv_done[j % kScoreTiles]);
+        }
+        __syncwarp();
+        if (j + 2 < n) {
+          if (kScoreTiles == 2) ok = all(products_done(j));  // with two, that of this one's
+          ok = ok && scores(j + 2);
+        }
       }
       // No product is left in flight when the operands and the tensor memory are given up, whatever ended the loop.
-      tc_commit(&sh.drained);
+      if (one) tc_commit(&sh.drained);
+      __syncwarp();
       ok = mbar_wait(&sh.drained, 0) && ok;
+      if (!ok) sh.failed = 1;
     }
     __syncwarp();
   } else {
     // ---------------------------------------------------------------- softmax: a row a lane, half of the positions
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 144;\n");
+    float row_m = -INFINITY, row_l = 0.f, row_b = 0.f;  // the row's maximum in use, sum, sum in units of V
+    int eref = -200;                                    // O is in units of 2^(eref - kTileShift)
     const int half = warp >> 2, quad = warp & 3, row = quad * 32 + lane;
     const uint32_t lanes = static_cast<uint32_t>(quad * 32) << 16;
-    const bool row_ok = row < nq;
-    const int qi = q0 + (row_ok ? row : 0), pos = row_ok ? sq.p0 + qi / p.group : -1;
+    const int pos = row < nq ? sq.p0 + (q0 + row) / p.group : -1;
     const bool idle = quad * 32 >= nq;  // no row of this warp is a query
-    float fq, hq;
     {
-      const float4* q = reinterpret_cast<const float4*>(
-          p.q + (static_cast<int64_t>(sq.r0 + qi / p.group) * p.n_head + kh * p.group + qi % p.group) * HD);
-      float top = 0.f, sum = 0.f;
-#pragma unroll 8
-      for (int i = 0; i < HD / 4; ++i) {
-        const float4 x = row_ok ? __ldcg(q + i) : make_float4(0.f, 0.f, 0.f, 0.f);
-        top = fmaxf(top, fmaxf(fmaxf(fabsf(x.x), fabsf(x.y)), fmaxf(fabsf(x.z), fabsf(x.w))));
-        sum += (x.x + x.y) + (x.z + x.w);
+      // Sixteen rows a warp, read whole into their place: scaled so that the largest magnitude is in [2^13, 2^14) and
+      // split; a negative factor of the scores changes the query's sign.  (Loops kept rolled: straight-line code that runs
+      // once a CTA is fetched from far.)
+      uint8_t* const stage = reinterpret_cast<uint8_t*>(sh.rows);
+      constexpr int kPitch = TileShared<HD>::kRow * 4;
+      if (lane < 16 && warp * 16 + lane < nq) {
+        const int qj = q0 + warp * 16 + lane;
+        sh.row_at[warp * 16 + lane] =
+            (static_cast<int64_t>(sq.r0 + qj / p.group) * p.n_head + kh * p.group + qj % p.group) * HD;
       }
-      // The largest magnitude goes to [2^13, 2^14); a negative factor of the scores changes the query's sign.
-      const int e = min(max(exponent_of(top), -100), 126);
-      const float up = p.scale < 0.f ? -pow2i(13 - e) : pow2i(13 - e);
-#pragma unroll 4
-      for (int i = half * (HD / 16); i < (half + 1) * (HD / 16); ++i) {
-        const float4 z = make_float4(0.f, 0.f, 0.f, 0.f);
-        const float4 a = row_ok ? __ldcg(q + 2 * i) : z, b = row_ok ? __ldcg(q + 2 * i + 1) : z;
-        uint4 h, l;
-        split2(a.x * up, a.y * up, h.x, l.x);
-        split2(a.z * up, a.w * up, h.y, l.y);
-        split2(b.x * up, b.y * up, h.z, l.z);
-        split2(b.z * up, b.w * up, h.w, l.w);
-        *reinterpret_cast<uint4*>(sh.q[0] + i * kChunkBytes + row * 16) = h;
-        *reinterpret_cast<uint4*>(sh.q[1] + i * kChunkBytes + row * 16) = l;
+      __syncwarp();
+#pragma unroll 1
+      for (int r = warp * 16; r < warp * 16 + 16; ++r) {
+        float4* to = reinterpret_cast<float4*>(stage + r * kPitch) + lane;
+        if (lane < HD / 4) {
+          if (r < nq)
+            cp_async16(to, reinterpret_cast<const float4*>(p.q + sh.row_at[r]) + lane);
+          else
+            *to = make_float4(0.f, 0.f, 0.f, 0.f);
+        }
       }
-      hq = 0.5f * up * sum;
-      fq = fabsf(p.scale) * kLog2e * pow2i(e - 13);
-      fence_async_smem();
+      cp_async_commit();
+      cp_async_wait<0>();
+      __syncwarp();
+#pragma unroll 2
+      for (int r = warp * 16; r < warp * 16 + 16; ++r) {
+        float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (lane < HD / 4) x = reinterpret_cast<const float4*>(stage + r * kPitch)[lane];
+        const float top = __uint_as_float(__reduce_max_sync(
+            0xffffffffu, __float_as_uint(fmaxf(fmaxf(fabsf(x.x), fabsf(x.y)), fmaxf(fabsf(x.z), fabsf(x.w))))));
+        const float sum = warp_sum((x.x + x.y) + (x.z + x.w));
+        const int e = min(max(exponent_of(top), -100), 126);
+        const float up = p.scale < 0.f ? -pow2i(13 - e) : pow2i(13 - e);
+        uint2 h, l;
+        split2(x.x * up, x.y * up, h.x, l.x);
+        split2(x.z * up, x.w * up, h.y, l.y);
+        if (lane < HD / 4) {  // every lane has read the row: the reductions are warp-wide
+          *reinterpret_cast<uint2*>(stage + r * kPitch + lane * 8) = h;
+          *reinterpret_cast<uint2*>(stage + r * kPitch + HD * 2 + lane * 8) = l;
+        }
+        if (lane == 0) {
+          sh.hq[r] = 0.5f * up * sum;
+          sh.fq[r] = fabsf(p.scale) * kLog2e * pow2i(e - 13);
+        }
+      }
+      asm volatile("bar.sync 1, 256;\n" ::: "memory");
+      // A row's high (half 0) or low parts to its lane.
+#pragma unroll 1
+      for (int i = 0; i < HD / 32; ++i) {
+        uint32_t v[16];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const uint4 y = *reinterpret_cast<const uint4*>(stage + row * kPitch + half * HD * 2 + i * 64 + k * 16);
+          v[4 * k] = y.x;
+          v[4 * k + 1] = y.y;
+          v[4 * k + 2] = y.z;
+          v[4 * k + 3] = y.w;
+        }
+        tc_st16(tmem + TileTmem<HD>::kQ + lanes + half * (HD / 2) + i * 16, v);
+      }
+      tc_wait_st();
+      tc_before();
       __syncwarp();
       if (lane == 0) mbar_arrive(&sh.q_full);
     }
-    for (int j = 0; j < n && ok; ++j) {
+    const float fq = sh.fq[row], hq = sh.hq[row];
+    // No softmax warp leaves the loop early, so that the pairs' barriers stay matched: after an expired wait it runs on
+    // without waiting.
+    for (int j = 0; j < n; ++j) {
       if (idle) {
         // In step with the others: the phase before must be over.
-        ok = j == 0 || mbar_wait(&sh.pv_done, static_cast<uint32_t>(j - 1) & 1u);
+        if (ok && j > 0) ok = products_done(j - 1);
         __syncwarp();
-        if (lane == 0) mbar_arrive(&sh.p_full);
+        if (lane == 0) mbar_arrive(&sh.p_full[j % kScoreTiles]);
         continue;
       }
-      ok = mbar_wait(&sh.scales[j & 3], static_cast<uint32_t>(j >> 2) & 1u) &&
-           mbar_wait(&sh.s_full[j & 1], static_cast<uint32_t>(j >> 1) & 1u);
-      if (__any_sync(0xffffffffu, !ok)) {
-        ok = false;
-        break;
-      }
+      ok = ok && mbar_wait(&sh.scales[j & 3], static_cast<uint32_t>(j >> 2) & 1u) &&
+           mbar_wait(&sh.s_full[j % kScoreTiles], static_cast<uint32_t>(j / kScoreTiles) & 1u);
+      __syncwarp();
       tc_after();
-      const uint32_t scol = tmem + kColS + (j & 1) * kTileK + lanes + half * kHalf;
+      const uint32_t scol = tmem + TileTmem<HD>::kS + (j % kScoreTiles) * kTileK + lanes + half * kHalf;
       uint32_t u[kHalf];
       tc_ld32(scol, u);
       tc_ld32(scol + 32, u + 32);
@@ -432,28 +537,28 @@ __global__ void __launch_bounds__(kTileThreads, 1) paged_tile_kernel(const Paged
                          (p.window == 0 || t0 > last_pos - p.window || t0 + kTileK <= p.n_sink);
       if (!plain) {
         const int h0 = t0 + half * kHalf;
-        const int hi = pos - h0;                                                       // columns above it are hidden,
-        const int low = p.window > 0 ? pos - p.window - h0 : -1, sk = p.n_sink - h0;  // up to `low` unless below `sk`
+        // Bit i: position h0 + i is seen.
+        auto up_to = [](int i) { return i < 0 ? 0ull : i >= 63 ? ~0ull : (2ull << i) - 1ull; };
+        uint64_t see = up_to(pos - h0);
+        if (p.window > 0) see &= ~up_to(pos - p.window - h0) | up_to(p.n_sink - 1 - h0);
+#pragma unroll
+        for (int b = 0; b < 4; ++b)
+          if (ve[b] == kHidden) see &= ~(0xffffull << (b * kSub));
+        const uint32_t bits[2] = {static_cast<uint32_t>(see), static_cast<uint32_t>(see >> 32)};
 #pragma unroll
         for (int i = 0; i < kHalf; ++i)
-          if (i > hi || (i <= low && i >= sk) || ve[i / kSub] == kHidden) x[i] = -INFINITY;
+          if ((bits[i >> 5] & (1u << (i & 31))) == 0u) x[i] = -INFINITY;
       }
       float top = -INFINITY;
 #pragma unroll
       for (int b = 0; b < 4; ++b) {
-        float t = x[b * kSub];
+        float t = fmaxf(x[b * kSub], x[b * kSub + 1]);
 #pragma unroll
-        for (int i = 1; i < kSub; ++i) t = fmaxf(t, x[b * kSub + i]);
+        for (int i = 2; i < kSub; i += 2) t = max3(t, x[b * kSub + i], x[b * kSub + i + 1]);
         top = fmaxf(top, (t + hq) * fmaxf(fq * ks[b], kLeast));
       }
       sh.top[j & 1][half][row] = top;
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&sh.maxima[quad]);
-      ok = mbar_wait(&sh.maxima[quad], static_cast<uint32_t>(j) & 1u);
-      if (__any_sync(0xffffffffu, !ok)) {
-        ok = false;
-        break;
-      }
+      asm volatile("bar.sync %0, 64;\n" ::"r"(2 + quad) : "memory");  // the other half's warp
       top = fmaxf(top, sh.top[j & 1][half ^ 1][row]);
       // The maximum in use follows the true one only when that is 2^8 above it; O follows then, and when V's scale grows.
       const bool grow = top > (row_m == -INFINITY ? row_m : row_m + kGrow);
@@ -469,21 +574,18 @@ __global__ void __launch_bounds__(kTileThreads, 1) paged_tile_kernel(const Paged
         row_b *= alpha;
         eref = en;
         if (j > 0) {
-          ok = mbar_wait(&sh.pv_done, static_cast<uint32_t>(j - 1) & 1u);
-          if (__any_sync(0xffffffffu, !ok)) {
-            ok = false;
-            break;
-          }
+          ok = ok && products_done(j - 1);
+          __syncwarp();
           tc_after();
 #pragma unroll
           for (int i = half * (HD / 32); i < (half + 1) * (HD / 32); ++i) {
             uint32_t o[16];
-            tc_ld16(tmem + kColO + lanes + i * 16, o);
+            tc_ld16(tmem + TileTmem<HD>::kO + lanes + i * 16, o);
             tc_wait_ld();
             tc_loaded16(o);
 #pragma unroll
             for (int k = 0; k < 16; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * alpha);
-            tc_st16(tmem + kColO + lanes + i * 16, o);
+            tc_st16(tmem + TileTmem<HD>::kO + lanes + i * 16, o);
           }
         }
       }
@@ -507,14 +609,21 @@ __global__ void __launch_bounds__(kTileThreads, 1) paged_tile_kernel(const Paged
           } else {
             off += static_cast<float>(eb);
           }
-          float sum = 0.f;
+          float2 sum2 = make_float2(0.f, 0.f);
+          const float2 a2 = make_float2(a, a), off2 = make_float2(off, off);
 #pragma unroll
           for (int i = 0; i < kSub / 2; ++i) {
             const int k = b * kSub + 2 * i;
-            const float w0 = exp2_fast(fmaf(x[k], a, off)), w1 = exp2_fast(fmaf(x[k + 1], a, off));
-            sum += w0 + w1;
-            split2(w0, w1, w[d * 8 + i], w[16 + d * 8 + i]);
+            const float2 y = fma2(make_float2(x[k], x[k + 1]), a2, off2);
+            const float2 e = make_float2(exp2_fast(y.x), exp2_fast(y.y));
+            sum2 = add2(sum2, e);
+            const __half2 h = __floats2half2_rn(e.x, e.y);
+            const float2 g = __half22float2(h), rest = fma2(g, make_float2(-1.f, -1.f), e);
+            const __half2 l = __floats2half2_rn(rest.x, rest.y);
+            w[d * 8 + i] = *reinterpret_cast<const uint32_t*>(&h);
+            w[16 + d * 8 + i] = *reinterpret_cast<const uint32_t*>(&l);
           }
+          const float sum = sum2.x + sum2.y;
           row_l += sum * pow2i(min(-eb, 60));
           row_b += sum;
         }
@@ -523,80 +632,75 @@ __global__ void __launch_bounds__(kTileThreads, 1) paged_tile_kernel(const Paged
       tc_wait_st();
       tc_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive(&sh.p_full);
+      if (lane == 0) mbar_arrive(&sh.p_full[j % kScoreTiles]);
     }
-    if (n > 0 && ok) ok = mbar_wait(&sh.pv_done, static_cast<uint32_t>(n - 1) & 1u);
+    if (n > 0 && ok) ok = products_done(n - 1);
+    if (__any_sync(0xffffffffu, !ok) && lane == 0) sh.failed = 1;
+    // Every product is done: the row's values in their own units.
+    __syncwarp();
+    tc_after();
     sh.l[half][row] = row_l;
     sh.b[half][row] = row_b;
-    tc_after();
-  }
-  if (!ok) sh.failed = 1;
-  if (lost && lane == 0) paged_error(p.rows);
-  // Every product is done (the softmax lanes waited for the last one); the operands' place holds the joined values.
-  tc_before();
-  __syncthreads();
-  tc_after();
-  float* part = reinterpret_cast<float*>(nrank > 1 ? sh.ring[0] : nullptr);  // [kTileQ][HD]
-  if (warp < 8) {
-    const int half = warp >> 2, row = (warp & 3) * 32 + lane;
-    const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
-    const int qi = q0 + row;
-    float* out = p.out + (static_cast<int64_t>(sq.r0 + qi / p.group) * p.n_head + kh * p.group + qi % p.group) * HD;
-    const float l = sh.l[0][row] + sh.l[1][row], b = 0.5f * (sh.b[0][row] + sh.b[1][row]);
-    const float unit = pow2i(max(eref, -126));
-    const float inv = nrank > 1 ? 1.f : l == 0.f ? 0.f : 1.f / l;
-    if (nrank > 1 && half == 0) sh.m[row] = row_m;
-#pragma unroll
+    if (half == 0) sh.m[row] = row_m;
+    asm volatile("bar.sync 1, 256;\n" ::: "memory");
+    const float b = 0.5f * (sh.b[0][row] + sh.b[1][row]), unit = pow2i(max(eref, -126));
+    const float l = sh.l[0][row] + sh.l[1][row], inv = nrank > 1 ? 1.f : l == 0.f ? 0.f : 1.f / l;
+#pragma unroll 1
     for (int i = half * (HD / 32); i < (half + 1) * (HD / 32); ++i) {
       uint32_t o[16];
       if (n > 0) {
-        tc_ld16(tmem + kColO + lanes + i * 16, o);
+        tc_ld16(tmem + TileTmem<HD>::kO + lanes + i * 16, o);
         tc_wait_ld();
         tc_loaded16(o);
       }
-      float4* to = reinterpret_cast<float4*>(nrank > 1 ? part + row * HD + i * 16 : out + i * 16);
-      if (row < nq) {
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          float v[4];
+      for (int k = 0; k < 4; ++k) {
+        float v[4];
 #pragma unroll
-          for (int e = 0; e < 4; ++e)
-            v[e] = n > 0 ? (__uint_as_float(o[4 * k + e]) + b) * pow2i(-kTileShift) * unit * inv : 0.f;
-          to[k] = make_float4(v[0], v[1], v[2], v[3]);
-        }
+        for (int e = 0; e < 4; ++e)
+          v[e] = n > 0 ? (__uint_as_float(o[4 * k + e]) + b) * pow2i(-kTileShift) * unit * inv : 0.f;
+        *reinterpret_cast<float4*>(&sh.rows[row][i * 16 + k * 4]) = make_float4(v[0], v[1], v[2], v[3]);
       }
     }
     tc_before();
   }
-  if (nrank > 1) {
+  if (nrank > 1)
     cluster.sync();
-    // Rows of the tile in turn over the ranks, joined in rank order.
-    for (int i = rank * kTileThreads + tid; i < nq * HD / 4; i += nrank * kTileThreads) {
-      const int row = i / (HD / 4), d = i % (HD / 4), qi = q0 + row;
-      float top = -INFINITY, sum = 0.f;
-      float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-      for (int r = 0; r < nrank; ++r) top = fmaxf(top, cluster.map_shared_rank(sh.m, r)[row]);
-      for (int r = 0; r < nrank; ++r) {
-        const float mr = cluster.map_shared_rank(sh.m, r)[row];
-        const float a = mr == -INFINITY ? 0.f : exp2_fast(mr - top);
-        const float4 y = reinterpret_cast<const float4*>(cluster.map_shared_rank(part, r))[i];
-        const float* lr = cluster.map_shared_rank(&sh.l[0][0], r);
-        sum += a * (lr[row] + lr[kTileQ + row]);
-        v.x += a * y.x;
-        v.y += a * y.y;
-        v.z += a * y.z;
-        v.w += a * y.w;
-      }
-      const float inv = sum == 0.f ? 0.f : 1.f / sum;
-      reinterpret_cast<float4*>(p.out + (static_cast<int64_t>(sq.r0 + qi / p.group) * p.n_head + kh * p.group +
-                                         qi % p.group) * HD)[d] = make_float4(v.x * inv, v.y * inv, v.z * inv, v.w * inv);
-    }
-    cluster.sync();  // no CTA leaves while another reads its part
-  } else {
+  else
     __syncthreads();
+  if (warp < 8) {
+    constexpr int kQuads = HD / 4;
+    if (nrank == 1) {
+#pragma unroll 4
+      for (int i = tid; i < nq * kQuads; i += kSoftThreads) {
+        const int row = i / kQuads, d = i % kQuads;
+        reinterpret_cast<float4*>(p.out + sh.row_at[row])[d] = reinterpret_cast<const float4*>(sh.rows[row])[d];
+      }
+    } else {
+      // Rows of the tile in turn over the ranks, joined in rank order.
+      for (int i = rank * kSoftThreads + tid; i < nq * kQuads; i += nrank * kSoftThreads) {
+        const int row = i / kQuads, d = i % kQuads;
+        float top = -INFINITY, sum = 0.f;
+        float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+        for (int r = 0; r < nrank; ++r) top = fmaxf(top, cluster.map_shared_rank(sh.m, r)[row]);
+        for (int r = 0; r < nrank; ++r) {
+          const TileShared<HD>* o = cluster.map_shared_rank(&sh, r);
+          const float a = o->m[row] == -INFINITY ? 0.f : exp2_fast(o->m[row] - top);
+          const float4 y = reinterpret_cast<const float4*>(o->rows[row])[d];
+          sum += a * (o->l[0][row] + o->l[1][row]);
+          v.x += a * y.x;
+          v.y += a * y.y;
+          v.z += a * y.z;
+          v.w += a * y.w;
+        }
+        const float inv = sum == 0.f ? 0.f : 1.f / sum;
+        reinterpret_cast<float4*>(p.out + sh.row_at[row])[d] = make_float4(v.x * inv, v.y * inv, v.z * inv, v.w * inv);
+      }
+    }
   }
+  if (nrank > 1) cluster.sync();  // no CTA leaves while another reads its part
   if (tid == 0 && sh.failed != 0 && p.rows.err != nullptr) atomicCAS(p.rows.err, 0, NH_E_TIMEOUT);
-  if (warp == 12) {
+  if (warp == 16) {
     tc_after();
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;\n" ::"r"(tmem), "r"(kTmemCols) : "memory");
   }

@@ -522,7 +522,7 @@ int nh_paged_read(const NhPagedKv* kv, const NhPagedRows* rows, int32_t out_type
  * A draft id outside [0, n_vocab) is refused; a row without mass draws id -1;
  * both record NH_E_ARG in *err (may be null).  So does a sequence with n < 0 or
  * n > max_draft or an offset outside [0, n_drafts]; nothing is written for it.
- * Every row is at most 2^31-1 ids long. */
+ * Every row is at most 2^30 ids long. */
 typedef struct NhVerifyDrafts {
   const float* target;    /* [n_drafts + n_seq] rows */
   int64_t target_stride;  /* floats between rows */

@@ -43,21 +43,6 @@ __device__ __forceinline__ SeqRows seq_rows(const PagedRows& r, int s, int64_t l
   return q;
 }
 
-// The sequence that row r belongs to: the last s with row_off[s] <= r, or -1
-// when r lies outside row_off[0] .. row_off[n_seq] - 1.
-__device__ __forceinline__ int seq_of_row(const PagedRows& rows, int r) {
-  int lo = 0, hi = rows.n_seq;  // row_off[lo] <= r < row_off[hi]
-  if (r < rows.row_off[0] || r >= rows.row_off[hi]) return -1;
-  while (hi - lo > 1) {
-    const int m = (lo + hi) >> 1;
-    if (rows.row_off[m] <= r)
-      lo = m;
-    else
-      hi = m;
-  }
-  return lo;
-}
-
 inline bool paged_aligned(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 
 // The host checks of the two argument blocks; fills the kernels' forms.

@@ -156,6 +156,7 @@ __global__ void __launch_bounds__(kVerifyThreads) verify_drafts_kernel(const NhV
     if (rank == 0 && tid == 0 && d.err != nullptr) atomicCAS(d.err, 0, NH_E_ARG);
     return;
   }
+  if (nrank > 1) cluster.barrier_arrive();  // the others must have started before their shared memory is written
   if (tid == 0) first = n;
   __syncthreads();
   const float* t0 = d.target + static_cast<int64_t>(o + s) * d.target_stride;
@@ -191,8 +192,10 @@ __global__ void __launch_bounds__(kVerifyThreads) verify_drafts_kernel(const NhV
     __syncthreads();
     if (warp == 0) {
       const double t = warp_sum_d(lane < kVerifyWarps ? wsum[lane] : 0.0);
+      if (nrank > 1 && pass == 0) cluster.barrier_wait();
       if (lane < nrank) cluster.map_shared_rank(&total[pass][0], lane)[rank] = t;
     }
+    if (nrank > 1 && pass == 0 && warp != 0) cluster.barrier_wait();
     if (nrank > 1)
       cluster.sync();
     else

@@ -2,7 +2,7 @@
 // positions and drafted ones (nh_paged_attention's split form).
 //
 // What bounds it: every cached byte is read once, so the copy rate of HBM.  A
-// CTA takes up to 4, 8 or 16 queries of one (sequence, KV head) and a contiguous
+// CTA takes up to 2, 4, 8 or 16 queries of one (sequence, KV head) and a contiguous
 // part of the positions; a cluster's CTAs split the positions and join their
 // (maximum, sum, weighted values) through distributed shared memory in rank
 // order.  A warp takes units of 16 positions, always inside one page, through a
@@ -10,6 +10,9 @@
 // warps), and reads them in the operand layout of mma.m16n8k16: both the
 // dimensions of K and those of V may be permuted freely, so each lane reads
 // whole 16-byte pieces.
+//   2 queries: the scores by integer products (m16n8k32), K's codes as they
+//   are: a query is scaled to 23-bit whole numbers, whose three balanced base-256
+//   digits are columns of B; sums exact, joined in f32.  Weights as below.
 //   4 queries: the codes are the A operand, the queries' (and weights') high
 //   and low parts the 8 columns of B; half the products and accumulators of the
 //   next form, four shuffles to bring the weights into place.
@@ -32,15 +35,23 @@ namespace {
 constexpr int kUnit = 16;  // positions of one warp step
 // Warps of a CTA: sixteen to an SM either way by their registers, in fewer and larger CTAs for four queries (one long
 // sequence 158 -> 135 us, the decode batch 134 -> 127 us against four warps a CTA).
-constexpr int kFewQueries = 16;
+constexpr int kFewQueries = 32;
 template <int NQ>
-constexpr int kWarpsOf = NQ == 4 ? 8 : 4;
+constexpr int kWarpsOf = NQ <= 4 ? 8 : 4;
 
 __device__ __forceinline__ void mma_f16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
                                         uint32_t b1) {
   asm volatile(
       "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};\n"
       : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+__device__ __forceinline__ void mma_u8s8(int (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                         uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k32.row.col.s32.u8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};\n"
+      : "+r"(d[0]), "+r"(d[1]), "+r"(d[2]), "+r"(d[3])
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
@@ -100,6 +111,7 @@ struct SplitShared {
   float m[kSplitWarps][NQ], l[kSplitWarps][NQ];
   float cm[NQ], cl[NQ];
   uint4 qa[NQ == 16 ? HD / 16 : 1][2][32];  // A operands of the 16-query form: high, low
+  uint32_t qd[NQ == 2 ? HD / 16 : 1][32];   // digits of the 2-query form
 };
 
 // Unit `i` of the visible ones: the sinks' units, then those from `lo` on.
@@ -116,8 +128,9 @@ __global__ void __launch_bounds__(kWarpsOf<NQ> * 32, NQ == 8 ? 3 : 2) paged_spli
   constexpr int KW = KV / 4, KN = HD / (4 * KV);  // words of such a piece, pieces a row
   constexpr int VW = HD / 32;                    // words of V a lane loads a row
   constexpr int QT = NQ == 16 ? 2 : 1;           // queries a lane holds scores of
-  constexpr int ST = NQ == 4 ? 2 : 4;            // scores a lane holds of each, a unit
-  constexpr int ON = NQ == 4 ? HD / 16 : HD / 8;  // accumulator tiles
+  constexpr bool kSmall = NQ <= 4;               // the codes are the A operand
+  constexpr int ST = kSmall ? 2 : 4;             // scores a lane holds of each, a unit
+  constexpr int ON = kSmall ? HD / 16 : HD / 8;  // accumulator tiles
   extern __shared__ __align__(16) uint8_t split_smem[];
   auto& sh = *reinterpret_cast<SplitShared<HD, NQ>*>(split_smem);
   cg::cluster_group cluster = cg::this_cluster();
@@ -209,12 +222,14 @@ __global__ void __launch_bounds__(kWarpsOf<NQ> * 32, NQ == 8 ? 3 : 2) paged_spli
 
   // The query's operand: word w of lane t holds dimensions dim(w) .. dim(w)+3.
   auto dim = [&](int w) { return (w / KW) * (4 * KV) + t * KV + (w % KW) * 4; };
-  uint32_t qa[NQ <= 8 ? KS : 1][4];
+  uint32_t qa[NQ == 4 || NQ == 8 ? KS : 1][4], qd[NQ == 2 ? KS : 1];
+  int h0 = 0, h1 = 0;            // 2 queries: 255 times the digit sums of this lane's two columns,
+  float m0 = 0.f, m1 = 0.f;      // and half of what their digits stand for
   float fq[QT], hq[QT];
   int pos[QT];
 #pragma unroll
   for (int k = 0; k < QT; ++k) {
-    const int jq = NQ == 4 ? g >> 1 : g + 8 * k;  // the query whose operand this lane holds
+    const int jq = NQ == 2 ? (g >> 1) & 1 : NQ == 4 ? g >> 1 : g + 8 * k;  // the query whose operand this lane holds
     const int j = q0 + jq;
     const bool ok = jq < nq;
     const int row = sq.r0 + (ok ? j / p.group : 0), head = kh * p.group + (ok ? j % p.group : 0);
@@ -229,8 +244,54 @@ __global__ void __launch_bounds__(kWarpsOf<NQ> * 32, NQ == 8 ? 3 : 2) paged_spli
     }
     top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
     top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-    // The largest magnitude goes to [2^13, 2^14).
     const int e = min(max(exponent_of(top), -100), 126);
+    if constexpr (NQ == 2) {
+      // Whole numbers of at most 2^22, column g: digit 0 or 1 of query (g / 2) % 2 for g < 4, else 2 (even) or none.  A
+      // warp forms its share of the words for all of them.
+      const float up = pow2i(21 - e);
+      float off = 0.f;  // a NaN where the query holds a value that is not finite
+      const int digit = g < 4 ? g & 1 : 2;
+#pragma unroll
+      for (int w = 0; w < KS; ++w) {
+        off += (x[w].x * 0.f + x[w].y * 0.f) + (x[w].z * 0.f + x[w].w * 0.f);
+        if (w % kSplitWarps == warp) {
+          const float y[4] = {x[w].x, x[w].y, x[w].z, x[w].w};
+          uint32_t word = 0u;
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            int v = __float2int_rn(y[i] * up);
+            const int d2 = static_cast<int8_t>(v & 255);
+            v = (v - d2) >> 8;
+            const int d1 = static_cast<int8_t>(v & 255);
+            const int d0 = (v - d1) >> 8;
+            const int d = g > 3 && (g & 1) != 0 ? 0 : digit == 0 ? d0 : digit == 1 ? d1 : d2;
+            word |= static_cast<uint32_t>(d & 255) << (8 * i);
+          }
+          sh.qd[w][lane] = word;
+        }
+      }
+      __syncthreads();
+      int sum = 0;
+#pragma unroll
+      for (int w = 0; w < KS; ++w) {
+        qd[w] = sh.qd[w][lane];
+        sum = __dp4a(static_cast<int>(qd[w]), 0x01010101, sum);
+      }
+      sum += __shfl_xor_sync(0xffffffffu, sum, 1);
+      sum += __shfl_xor_sync(0xffffffffu, sum, 2);
+      off += __shfl_xor_sync(0xffffffffu, off, 1);
+      off += __shfl_xor_sync(0xffffffffu, off, 2);
+      // Scores: columns 2 t and 2 t + 1, query t % 2.
+      h0 = 255 * __shfl_sync(0xffffffffu, sum, 8 * t);
+      h1 = 255 * __shfl_sync(0xffffffffu, sum, 8 * t + 4);
+      m0 = t < 2 ? 32768.f : 0.5f;
+      m1 = t < 2 ? 128.f : 0.f;
+      hq[k] = __shfl_sync(0xffffffffu, off, 8 * (t & 1));
+      fq[k] = __shfl_sync(0xffffffffu, p.scale * kLog2e * pow2i(e - 21), 8 * (t & 1));
+      pos[k] = __shfl_sync(0xffffffffu, pos[k], 8 * (t & 1));
+      continue;
+    }
+    // The largest magnitude goes to [2^13, 2^14).
     const float up = pow2i(13 - e);
     float sum = 0.f;
 #pragma unroll
@@ -300,8 +361,19 @@ __global__ void __launch_bounds__(kWarpsOf<NQ> * 32, NQ == 8 ? 3 : 2) paged_spli
     float c[2][4];  // two chains of products: of even and odd k-steps (4 queries), of positions 0-7 and 8-15 (others)
 #pragma unroll
     for (int j = 0; j < 2; ++j) c[j][0] = c[j][1] = c[j][2] = c[j][3] = 0.f;
+    if constexpr (NQ == 2) {
+      int ci[4] = {0, 0, 0, 0};
 #pragma unroll
-    for (int w = 0; w < KS; ++w) {
+      for (int w = 0; w < KS; w += 2) mma_u8s8(ci, kw[0][w], kw[1][w], kw[0][w + 1], kw[1][w + 1], qd[w], qd[w + 1]);
+      // Twice the digits' products with the codes' own values (u - 127.5), whole and exact; then the digits' weights.
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const float part = fmaf(static_cast<float>(2 * ci[2 * e] - h0), m0, static_cast<float>(2 * ci[2 * e + 1] - h1) * m1);
+        c[0][e] = part + __shfl_xor_sync(0xffffffffu, part, 2);
+      }
+    }
+#pragma unroll
+    for (int w = 0; w < (NQ == 2 ? 0 : KS); ++w) {
       const uint32_t a0 = codes_lo(kw[0][w]), a1 = codes_hi(kw[0][w]), b0 = codes_lo(kw[1][w]), b1 = codes_hi(kw[1][w]);
       if constexpr (NQ == 4) {
         mma_f16(c[w & 1], a0, b0, a1, b1, qa[w][0], qa[w][1]);
@@ -326,7 +398,8 @@ __global__ void __launch_bounds__(kWarpsOf<NQ> * 32, NQ == 8 ? 3 : 2) paged_spli
       const float f = fq[k] * k_scale;
 #pragma unroll
       for (int e = 0; e < ST; ++e) {
-        const float d = NQ == 4   ? (c[0][2 * e] + c[1][2 * e]) + (c[0][2 * e + 1] + c[1][2 * e + 1])
+        const float d = NQ == 2   ? c[0][e]
+                        : NQ == 4 ? (c[0][2 * e] + c[1][2 * e]) + (c[0][2 * e + 1] + c[1][2 * e + 1])
                         : NQ == 8 ? c[e >> 1][e & 1] + c[e >> 1][(e & 1) + 2]
                                   : c[e >> 1][2 * k + (e & 1)];
         x[k][e] = (d + hq[k]) * f;
@@ -334,7 +407,7 @@ __global__ void __launch_bounds__(kWarpsOf<NQ> * 32, NQ == 8 ? 3 : 2) paged_spli
       if (!plain) {
 #pragma unroll
         for (int e = 0; e < ST; ++e) {
-          const int tk = t0 + (NQ == 4 ? g + 8 * e : 8 * (e >> 1) + 2 * t + (e & 1));
+          const int tk = t0 + (kSmall ? g + 8 * e : 8 * (e >> 1) + 2 * t + (e & 1));
           if (!seen_here || tk > pos[k] || (p.window != 0 && tk <= pos[k] - p.window && tk >= p.n_sink))
             x[k][e] = -INFINITY;
         }
@@ -343,7 +416,7 @@ __global__ void __launch_bounds__(kWarpsOf<NQ> * 32, NQ == 8 ? 3 : 2) paged_spli
 #pragma unroll
       for (int e = 0; e < ST; ++e) top[k] = fmaxf(top[k], x[k][e]);
 #pragma unroll
-      for (int e = NQ == 4 ? 4 : 1; e <= (NQ == 4 ? 16 : 2); e <<= 1)
+      for (int e = kSmall ? 4 : 1; e <= (kSmall ? 16 : 2); e <<= 1)
         top[k] = fmaxf(top[k], __shfl_xor_sync(0xffffffffu, top[k], e));
       grew |= top[k] > m[k];
     }
@@ -386,15 +459,16 @@ __global__ void __launch_bounds__(kWarpsOf<NQ> * 32, NQ == 8 ? 3 : 2) paged_spli
         w[e] *= fw;
         b[k] += w[e];
       }
-      if constexpr (NQ == 4) {
+      if constexpr (kSmall) {
         // Column g of B: query g / 2's weights at positions 2 t, 2 t + 1 and 8 further, from the lanes that hold them.
         const int from = 8 * t + (g >> 1);
         const float w0 = __shfl_sync(0xffffffffu, w[0], from), w1 = __shfl_sync(0xffffffffu, w[0], from + 4);
         const float w2 = __shfl_sync(0xffffffffu, w[1], from), w3 = __shfl_sync(0xffffffffu, w[1], from + 4);
-        w[0] = w0;
-        w[1] = w1;
-        w[2] = w2;
-        w[3] = w3;
+        const bool used = NQ == 4 || g < 4;
+        w[0] = used ? w0 : 0.f;
+        w[1] = used ? w1 : 0.f;
+        w[2] = used ? w2 : 0.f;
+        w[3] = used ? w3 : 0.f;
       }
       split2(w[0], w[1], hi[k][0], lo[k][0]);
       split2(w[2], w[3], hi[k][1], lo[k][1]);
@@ -409,7 +483,7 @@ __global__ void __launch_bounds__(kWarpsOf<NQ> * 32, NQ == 8 ? 3 : 2) paged_spli
       const uint32_t b01 = __byte_perm(vw[2][w], vw[3][w], 0x5140), b23 = __byte_perm(vw[2][w], vw[3][w], 0x7362);
       const uint32_t va[4] = {codes_lo(a01), codes_hi(a01), codes_lo(a23), codes_hi(a23)};
       const uint32_t vb[4] = {codes_lo(b01), codes_hi(b01), codes_lo(b23), codes_hi(b23)};
-      if constexpr (NQ == 4) {
+      if constexpr (kSmall) {
 #pragma unroll
         for (int e = 0; e < 2; ++e) mma_f16(o[2 * w + e], va[2 * e], va[2 * e + 1], vb[2 * e], vb[2 * e + 1], b0, b1);
       } else {
@@ -434,12 +508,13 @@ __global__ void __launch_bounds__(kWarpsOf<NQ> * 32, NQ == 8 ? 3 : 2) paged_spli
 #pragma unroll
   for (int k = 0; k < QT; ++k) {
 #pragma unroll
-    for (int e = NQ == 4 ? 4 : 1; e <= (NQ == 4 ? 16 : 2); e <<= 1) {
+    for (int e = kSmall ? 4 : 1; e <= (kSmall ? 16 : 2); e <<= 1) {
       l[k] += __shfl_xor_sync(0xffffffffu, l[k], e);
       b[k] += __shfl_xor_sync(0xffffffffu, b[k], e);
     }
-    const int qk = NQ == 4 ? t : g + 8 * k;
-    if (NQ == 4 ? g == 0 : t == 0) {
+    const int qk = kSmall ? t : g + 8 * k;
+    if (kSmall && t >= NQ) continue;  // columns without a query
+    if (kSmall ? g == 0 : t == 0) {
       sh.m[warp][qk] = m[k];
       sh.l[warp][qk] = l[k];
     }
@@ -447,8 +522,8 @@ __global__ void __launch_bounds__(kWarpsOf<NQ> * 32, NQ == 8 ? 3 : 2) paged_spli
     for (int n = 0; n < ON; ++n)
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
-        const float v = NQ == 4 ? o[n][2 * e] + o[n][2 * e + 1] : NQ == 8 ? o[n][e] + o[n][e + 2] : o[n][2 * k + e];
-        const int d = NQ == 4 ? g * VW * 4 + 2 * n + e : (2 * t + e) * VW * 4 + n;
+        const float v = kSmall ? o[n][2 * e] + o[n][2 * e + 1] : NQ == 8 ? o[n][e] + o[n][e + 2] : o[n][2 * k + e];
+        const int d = kSmall ? g * VW * 4 + 2 * n + e : (2 * t + e) * VW * 4 + n;
         sh.o[warp][qk][d] = (v + 0.5f * b[k]) * pow2i(-kWeightShift) * unit;
       }
   }
@@ -504,19 +579,26 @@ int launch_split(const PagedAttnArgs& p, int groups, int ranks, cudaStream_t s) 
                         dim3(kWarpsOf<NQ> * 32), ranks, smem, s, p);
 }
 
-template <int HD>
-int launch_split_hd(const PagedAttnArgs& p, cudaStream_t s) {
-  const int64_t most = std::min<int64_t>(p.few, static_cast<int64_t>(p.rows.max_rows) * p.group);
-  const int nq = most <= 4 ? 4 : most <= 8 ? 8 : 16, groups = static_cast<int>((most + nq - 1) / nq);
+// CTAs of a (sequence, KV head, query group): one, unless the groups alone leave SMs empty.  (More are not free: each
+// forms the query's operand and joins what it has; 16 sequences' 20 queries to 6001 positions take 88 us with 4, 112 with 8.)
+template <int HD, int NQ>
+int launch_group(const PagedAttnArgs& p, int groups, cudaStream_t s) {
   if (static_cast<int64_t>(p.kv.n_kv) * groups > 65535) return NH_E_ARG;
+  constexpr int kWarps = kWarpsOf<NQ>;
   const int64_t items = static_cast<int64_t>(p.rows.n_seq) * p.kv.n_kv * groups;
   const int64_t units = static_cast<int64_t>(p.rows.max_blocks) * p.kv.page / kUnit;
-  const int warps = nq == 4 ? kWarpsOf<4> : kWarpsOf<16>;
   int ranks = 1;
-  while (ranks < 16 && items * ranks * warps < 16 * device_sm_count() && units > 2 * warps * ranks) ranks *= 2;
-  return nq == 4   ? launch_split<HD, 4>(p, groups, ranks, s)
-         : nq == 8 ? launch_split<HD, 8>(p, groups, ranks, s)
-                   : launch_split<HD, 16>(p, groups, ranks, s);
+  while (ranks < 16 && items * ranks * kWarps < 16 * device_sm_count() && units > 2 * kWarps * ranks) ranks *= 2;
+  return launch_split<HD, NQ>(p, groups, ranks, s);
+}
+
+template <int HD>
+int launch_split_hd(const PagedAttnArgs& p, cudaStream_t s) {
+  const int most = static_cast<int>(std::min<int64_t>(p.few, static_cast<int64_t>(p.rows.max_rows) * p.group));
+  return most <= 2   ? launch_group<HD, 2>(p, 1, s)
+         : most <= 4 ? launch_group<HD, 4>(p, 1, s)
+         : most <= 8 ? launch_group<HD, 8>(p, 1, s)
+                     : launch_group<HD, 16>(p, (most + 15) / 16, s);
 }
 
 }  // namespace

@@ -58,12 +58,11 @@ struct TileShared {
   static constexpr int kOperand = HD / 8 * kChunkBytes, kScoreTiles = TileTmem<HD>::kScoreTiles;
   static constexpr int kRow = HD + 4;  // floats of a joined row, padded against bank conflicts
   uint8_t ring[2][2][kOperand];        // K, V: two stages each
-  // Q's parts on their way to tensor memory ([row][high, low] f16); the joined values once the products are done.
+  // Q on its way to tensor memory; the joined values once the products are done.
   float rows[kTileQ][kRow];
   float ks[4][kSubs];  // scales of a tile's 16-position parts (four tiles)
   int ve[4][kSubs];    // exponents of V's, or kHidden
   float top[2][2][kTileQ];  // the halves' maxima of a row (two tiles)
-  float fq[kTileQ], hq[kTileQ];
   int64_t row_at[kTileQ];  // where a query's row starts in q and out
   uint64_t full[2][2], empty[2][2], scales[4], q_full, s_full[kScoreTiles], p_full[kScoreTiles], pv_done[kScoreTiles], drained;
   float m[kTileQ], l[2][kTileQ], b[2][kTileQ];
@@ -435,12 +434,11 @@ __global__ void __launch_bounds__(kTileThreads, 1) paged_tile_kernel(const Paged
     const uint32_t lanes = static_cast<uint32_t>(quad * 32) << 16;
     const int pos = row < nq ? sq.p0 + (q0 + row) / p.group : -1;
     const bool idle = quad * 32 >= nq;  // no row of this warp is a query
+    float fq, hq;
     {
-      // Sixteen rows a warp, read whole into their place: scaled so that the largest magnitude is in [2^13, 2^14) and
-      // split; a negative factor of the scores changes the query's sign.  (Loops kept rolled: straight-line code that runs
-      // once a CTA is fetched from far.)
-      uint8_t* const stage = reinterpret_cast<uint8_t*>(sh.rows);
-      constexpr int kPitch = TileShared<HD>::kRow * 4;
+      // The rows, read whole; then a lane scales its own so that the largest magnitude is in [2^13, 2^14), and splits it:
+      // the high parts by half 0, the low ones by half 1.  A negative factor of the scores changes the query's sign.
+      // (Loops kept rolled: straight-line code that runs once a CTA is fetched from far.)
       if (lane < 16 && warp * 16 + lane < nq) {
         const int qj = q0 + warp * 16 + lane;
         sh.row_at[warp * 16 + lane] =
@@ -449,7 +447,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) paged_tile_kernel(const Paged
       __syncwarp();
 #pragma unroll 1
       for (int r = warp * 16; r < warp * 16 + 16; ++r) {
-        float4* to = reinterpret_cast<float4*>(stage + r * kPitch) + lane;
+        float4* to = reinterpret_cast<float4*>(sh.rows[r]) + lane;
         if (lane < HD / 4) {
           if (r < nq)
             cp_async16(to, reinterpret_cast<const float4*>(p.q + sh.row_at[r]) + lane);
@@ -459,49 +457,38 @@ __global__ void __launch_bounds__(kTileThreads, 1) paged_tile_kernel(const Paged
       }
       cp_async_commit();
       cp_async_wait<0>();
-      __syncwarp();
-#pragma unroll 2
-      for (int r = warp * 16; r < warp * 16 + 16; ++r) {
-        float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
-        if (lane < HD / 4) x = reinterpret_cast<const float4*>(stage + r * kPitch)[lane];
-        const float top = __uint_as_float(__reduce_max_sync(
-            0xffffffffu, __float_as_uint(fmaxf(fmaxf(fabsf(x.x), fabsf(x.y)), fmaxf(fabsf(x.z), fabsf(x.w))))));
-        const float sum = warp_sum((x.x + x.y) + (x.z + x.w));
-        const int e = min(max(exponent_of(top), -100), 126);
-        const float up = p.scale < 0.f ? -pow2i(13 - e) : pow2i(13 - e);
-        uint2 h, l;
-        split2(x.x * up, x.y * up, h.x, l.x);
-        split2(x.z * up, x.w * up, h.y, l.y);
-        if (lane < HD / 4) {  // every lane has read the row: the reductions are warp-wide
-          *reinterpret_cast<uint2*>(stage + r * kPitch + lane * 8) = h;
-          *reinterpret_cast<uint2*>(stage + r * kPitch + HD * 2 + lane * 8) = l;
-        }
-        if (lane == 0) {
-          sh.hq[r] = 0.5f * up * sum;
-          sh.fq[r] = fabsf(p.scale) * kLog2e * pow2i(e - 13);
-        }
-      }
       asm volatile("bar.sync 1, 256;\n" ::: "memory");
-      // A row's high (half 0) or low parts to its lane.
+      const float4* mine = reinterpret_cast<const float4*>(sh.rows[row]);
+      float top = 0.f, sum = 0.f;
+#pragma unroll 4
+      for (int i = 0; i < HD / 4; ++i) {
+        const float4 x = mine[i];
+        top = max3(top, max3(fabsf(x.x), fabsf(x.y), fabsf(x.z)), fabsf(x.w));
+        sum += (x.x + x.y) + (x.z + x.w);
+      }
+      const int e = min(max(exponent_of(top), -100), 126);
+      const float up = p.scale < 0.f ? -pow2i(13 - e) : pow2i(13 - e);
 #pragma unroll 1
       for (int i = 0; i < HD / 32; ++i) {
         uint32_t v[16];
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          const uint4 y = *reinterpret_cast<const uint4*>(stage + row * kPitch + half * HD * 2 + i * 64 + k * 16);
-          v[4 * k] = y.x;
-          v[4 * k + 1] = y.y;
-          v[4 * k + 2] = y.z;
-          v[4 * k + 3] = y.w;
+        for (int k = 0; k < 8; ++k) {
+          const float4 x = mine[i * 8 + k];
+          uint32_t h0, l0, h1, l1;
+          split2(x.x * up, x.y * up, h0, l0);
+          split2(x.z * up, x.w * up, h1, l1);
+          v[2 * k] = half == 0 ? h0 : l0;
+          v[2 * k + 1] = half == 0 ? h1 : l1;
         }
         tc_st16(tmem + TileTmem<HD>::kQ + lanes + half * (HD / 2) + i * 16, v);
       }
+      hq = 0.5f * up * sum;
+      fq = fabsf(p.scale) * kLog2e * pow2i(e - 13);
       tc_wait_st();
       tc_before();
       __syncwarp();
       if (lane == 0) mbar_arrive(&sh.q_full);
     }
-    const float fq = sh.fq[row], hq = sh.hq[row];
     // No softmax warp leaves the loop early, so that the pairs' barriers stay matched: after an expired wait it runs on
     // without waiting.
     for (int j = 0; j < n; ++j) {

@@ -14,11 +14,12 @@
 // tensor cores form the scores ahead while weights are in the making.
 // What bounds it: the two-part products make 8 hd products a score and row
 // where one f16 pass would make 4 (the price of f32 queries and weights); beside
-// them some 8 operations a score for the softmax.  Operands lie in shared
-// memory as [8-dimension chunk][row][16 bytes], unswizzled: the same image
-// serves K (K-major) and V (MN-major), and eight lanes write 128 contiguous
-// bytes.  (Unswizzled operands are read at half the shared-memory rate: with Q
-// in shared memory too, a 16-wide step of the scores took 138 cycles for 64.)
+// them some 8 operations a score for the softmax.  Operand tiles lie in shared
+// memory as rows of 64 dimensions, 128 bytes swizzled: the same image serves K
+// (K-major) and V (MN-major), and eight lanes write to different banks.
+// (Unswizzled operands are read at half the rate: with Q in shared memory too, a
+// 16-wide step of the scores took 138 cycles for 64, and the softmax warps'
+// own accesses waited.)
 // All waits are bounded; an expired one records NH_E_TIMEOUT.
 #include <cooperative_groups.h>
 
@@ -39,7 +40,7 @@ constexpr int kSoftThreads = 256;
 constexpr int kHalf = kTileK / 2;  // positions of a tile that one softmax warp takes
 constexpr float kLeast = 1.17549435e-38f;  // factor of the scores at least: a hidden one, -inf, stays that
 constexpr int kHidden = -1000;     // V's exponent where no position is seen
-constexpr int kChunkBytes = kTileK * 16;  // one 8-dimension chunk of an operand tile
+constexpr int kHalfBytes = kTileK * 128;  // 64 dimensions of an operand tile
 constexpr int kTileShift = 7;   // weights are 2^7 times [0, 2^8]
 constexpr float kGrow = 8.f;    // the maximum in use lags the true one by at most 2^8
 
@@ -55,7 +56,7 @@ struct TileTmem {
 
 template <int HD>
 struct TileShared {
-  static constexpr int kOperand = HD / 8 * kChunkBytes, kScoreTiles = TileTmem<HD>::kScoreTiles;
+  static constexpr int kOperand = (HD + 63) / 64 * kHalfBytes, kScoreTiles = TileTmem<HD>::kScoreTiles;
   static constexpr int kRow = HD + 4;  // floats of a joined row, padded against bank conflicts
   uint8_t ring[2][2][kOperand];        // K, V: two stages each
   // Q on its way to tensor memory; the joined values once the products are done.
@@ -81,10 +82,12 @@ __device__ __forceinline__ void tc_commit(uint64_t* bar) {
                : "memory");
 }
 
-// Shared-memory operand descriptor, no swizzle, version 1.
-__device__ __forceinline__ uint64_t operand(uint32_t addr, uint32_t lead, uint32_t stride) {
+// Shared-memory operand descriptor, 128-byte swizzle, version 1: 8-row groups
+// 1024 bytes apart (K's rows of the score product, V's positions); `lead`: from
+// 64 columns of an MN-major operand to the next.
+__device__ __forceinline__ uint64_t operand(uint32_t addr, uint32_t lead) {
   return static_cast<uint64_t>((addr >> 4) & 0x3FFFu) | (static_cast<uint64_t>(lead >> 4) << 16) |
-         (static_cast<uint64_t>(stride >> 4) << 32) | (1ull << 46);
+         (static_cast<uint64_t>(1024 >> 4) << 32) | (1ull << 46) | (2ull << 61);
 }
 // Instruction descriptor: D f32, A and B f16, M = 128; B MN-major for V.
 __host__ __device__ constexpr uint32_t idesc(int n, bool mn_major) {
@@ -282,7 +285,9 @@ __global__ void __launch_bounds__(kTileThreads, 1) paged_tile_kernel(const Paged
   if (warp >= 8 && warp < 16) {
     // ---------------------------------------------------------------- codes to operands
     asm volatile("setmaxnreg.dec.sync.aligned.u32 72;\n");
-    const int of_v = (warp - 8) >> 2, w = warp & 3, r = lane & 7, c = lane >> 3;
+    // Lanes: row r of eight, 16-byte column c of four.  (Rows across neighbouring lanes instead cost eight times the load
+    // wavefronts, and with them a third of the kernel's time: they delay the softmax warps' tensor-memory loads.)
+    const int of_v = (warp - 8) >> 2, w = warp & 3, r = lane >> 2, c = lane & 3;
     const uint8_t* codes = (of_v ? p.kv.v_codes : p.kv.k_codes) + static_cast<uint64_t>(kh) * static_cast<uint32_t>(page * HD);
     const uint32_t page_bytes = static_cast<uint32_t>(p.kv.n_kv) * static_cast<uint32_t>(page * HD);  // at most 2^30
     const int32_t* table = p.rows.page_table + static_cast<int64_t>(s) * p.rows.max_blocks;
@@ -342,13 +347,15 @@ __global__ void __launch_bounds__(kTileThreads, 1) paged_tile_kernel(const Paged
       lost |= id0 == -2 || id1 == -2;
       ok = all(mbar_wait(&sh.empty[of_v][j & 1], static_cast<uint32_t>((j >> 1) & 1) ^ 1u));
       if (!ok) break;
-      uint8_t* to = sh.ring[of_v][j & 1] + (w * 32 + r) * 16;
+      uint8_t* to = sh.ring[of_v][j & 1] + (w * 32 + r) * 128;
 #pragma unroll
       for (int i = 0; i < kItems; ++i) {
-        uint8_t* d = to + rg_of(i) * 128 + col_of(i) * 2 * kChunkBytes;
-        *reinterpret_cast<uint4*>(d) =
+        // Two 8-dimension pieces of the row, which the swizzle moves by the row's place among eight.
+        const int col = col_of(i), piece = col * 2 & 7;
+        uint8_t* d = to + rg_of(i) * 1024 + (col >> 2) * kHalfBytes;
+        *reinterpret_cast<uint4*>(d + (piece ^ r) * 16) =
             make_uint4(codes_lo(raw[i].x), codes_hi(raw[i].x), codes_lo(raw[i].y), codes_hi(raw[i].y));
-        *reinterpret_cast<uint4*>(d + kChunkBytes) =
+        *reinterpret_cast<uint4*>(d + ((piece + 1) ^ r) * 16) =
             make_uint4(codes_lo(raw[i].z), codes_hi(raw[i].z), codes_lo(raw[i].w), codes_hi(raw[i].w));
       }
       // The scales' place was last read for tile j - 4, whose weights were in use before K of tile j found its stage free.
@@ -371,10 +378,12 @@ __global__ void __launch_bounds__(kTileThreads, 1) paged_tile_kernel(const Paged
     asm volatile("setmaxnreg.dec.sync.aligned.u32 48;\n");
     if (warp == 16 && n > 0) {
       constexpr uint32_t kOp = TileShared<HD>::kOperand;
-      constexpr uint64_t kStepK = 2 * kChunkBytes >> 4, kStepV = 256 >> 4;  // 16 dimensions of Q and K, 16 positions of V
+      // 16 dimensions of K (step k of its 64), 16 positions of V.
+      auto step_k = [](int k) { return static_cast<uint64_t>((k >> 2) * kHalfBytes + (k & 3) * 32) >> 4; };
+      constexpr uint64_t kStepV = 2048 >> 4;
       const bool one = elect_one();
-      const uint64_t kd = operand(smem_u32(sh.ring[0][0]), kChunkBytes, 128);
-      const uint64_t vd = operand(smem_u32(sh.ring[1][0]), 128, kChunkBytes);
+      const uint64_t kd = operand(smem_u32(sh.ring[0][0]), 16);
+      const uint64_t vd = operand(smem_u32(sh.ring[1][0]), kHalfBytes);
       const uint32_t qa = tmem + TileTmem<HD>::kQ, oa = tmem + TileTmem<HD>::kO;
       auto scores = [&](int j) {
         if (!all(mbar_wait(&sh.full[0][j & 1], static_cast<uint32_t>(j >> 1) & 1u))) return false;
@@ -384,7 +393,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) paged_tile_kernel(const Paged
         if (one) {
 #pragma unroll
           for (int k = 0; k < HD / 8; ++k)  // the high parts' steps, then the low ones'
-            mma_ts<idesc(kTileK, false)>(d, qa + k * 8, b + (k % (HD / 16)) * kStepK, k > 0 ? 1u : 0u);
+            mma_ts<idesc(kTileK, false)>(d, qa + k * 8, b + step_k(k % (HD / 16)), k > 0 ? 1u : 0u);
           tc_commit(&sh.empty[0][j & 1]);
           tc_commit(&sh.s_full[j % kScoreTiles]);
         }

@@ -39,7 +39,7 @@ struct AppendArgs {
   const float* q_norm;
   const float* k_norm;
   float eps;
-  int n_head, rope_len;
+  int n_head, rope_len, kv_per, q_per;  // heads of a CTA
   const float* rope_cs;
   float* qr;
 };
@@ -194,7 +194,7 @@ __global__ void __launch_bounds__(AppendShape<PAGE>::kThreads, 1024 / AppendShap
   if (!page_ok && rank == 0 && tid == 0) paged_error(p.rows);
 
   // This CTA's heads.
-  const int kv_per = (p.kv.n_kv + nrank - 1) / nrank, q_per = (p.n_head + nrank - 1) / nrank;
+  const int kv_per = p.kv_per, q_per = p.q_per;
   const int kh0 = min(rank * kv_per, p.kv.n_kv), kh1 = min(kh0 + kv_per, p.kv.n_kv);
   const int qh0 = min(rank * q_per, p.n_head), qh1 = min(qh0 + q_per, p.n_head);
   const bool has_q = p.q != nullptr, norm = p.k_norm != nullptr;
@@ -518,6 +518,8 @@ extern "C" int nh_paged_append(const NhPagedKv* kv, const NhPagedRows* rows, con
   // for any number of heads).
   int ranks = std::min(kMaxRanks, p.kv.n_kv);
   if (ranks == kMaxRanks && pages * p.rows.n_seq > 200) ranks = 4;
+  p.kv_per = (p.kv.n_kv + ranks - 1) / ranks;
+  p.q_per = (n_head + ranks - 1) / ranks;
   const unsigned np = static_cast<unsigned>(pages);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   switch (p.kv.hd) {

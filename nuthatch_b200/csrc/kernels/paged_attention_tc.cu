@@ -146,6 +146,10 @@ __device__ __forceinline__ void tc_st16(uint32_t addr, const uint32_t* v) {
       NH_W8(v, 8), "r"(addr)
       : "memory");
 }
+__device__ __forceinline__ void tc_st8(uint32_t addr, const uint32_t* v) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%8], {%0,%1,%2,%3,%4,%5,%6,%7};\n" ::NH_W8(v, 0), "r"(addr)
+               : "memory");
+}
 __device__ __forceinline__ void tc_loaded16(uint32_t* v) { asm volatile("" : NH_RW8(v, 0), NH_RW8(v, 8)); }
 __device__ __forceinline__ void tc_loaded(uint32_t* v) {
   asm volatile("" : NH_RW8(v, 0), NH_RW8(v, 8), NH_RW8(v, 16), NH_RW8(v, 24));
@@ -271,8 +275,8 @@ __global__ void __launch_bounds__(kTileThreads, 1) paged_tile_kernel(const Paged
   const int lo = p.window > 0 ? max(0, first_pos - p.window + 1) / kTileK : 0;
   const int n_sink = p.window > 0 ? min((min(p.n_sink, last_pos + 1) + kTileK - 1) / kTileK, lo) : 0;
   const int n_all = n_sink + last_pos / kTileK + 1 - lo;
-  const int j0 = static_cast<int>(static_cast<int64_t>(n_all) * rank / nrank);
-  const int n = static_cast<int>(static_cast<int64_t>(n_all) * (rank + 1) / nrank) - j0;
+  const int share = n_all / nrank, rest = n_all % nrank;
+  const int j0 = rank * share + min(rank, rest), n = share + (rank < rest ? 1 : 0);
   auto tile_pos = [&](int j) { return (j0 + j < n_sink ? j0 + j : j0 + j - n_sink + lo) * kTileK; };
 
   // Barriers.  A wait tells a phase's parity from the next one's only, so none may run two phases ahead of a waiter: one
@@ -445,21 +449,21 @@ __global__ void __launch_bounds__(kTileThreads, 1) paged_tile_kernel(const Paged
     const bool idle = quad * 32 >= nq;  // no row of this warp is a query
     float fq, hq;
     {
-      // The rows, read whole; then a lane scales its own so that the largest magnitude is in [2^13, 2^14), and splits it:
-      // the high parts by half 0, the low ones by half 1.  A negative factor of the scores changes the query's sign.
-      // (Loops kept rolled: straight-line code that runs once a CTA is fetched from far.)
+      // The rows, read whole; then the two lanes of a row scale half of it each so that the largest magnitude is in
+      // [2^13, 2^14), and split it.  A negative factor of the scores changes the query's sign.
+      int64_t at = 0;
       if (lane < 16 && warp * 16 + lane < nq) {
-        const int qj = q0 + warp * 16 + lane;
-        sh.row_at[warp * 16 + lane] =
-            (static_cast<int64_t>(sq.r0 + qj / p.group) * p.n_head + kh * p.group + qj % p.group) * HD;
+        const int qj = q0 + warp * 16 + lane, qr = qj / p.group;
+        at = (static_cast<int64_t>(sq.r0 + qr) * p.n_head + kh * p.group + qj - qr * p.group) * HD;
+        sh.row_at[warp * 16 + lane] = at;
       }
-      __syncwarp();
-#pragma unroll 1
-      for (int r = warp * 16; r < warp * 16 + 16; ++r) {
-        float4* to = reinterpret_cast<float4*>(sh.rows[r]) + lane;
+#pragma unroll 4
+      for (int i = 0; i < 16; ++i) {
+        const int64_t from = __shfl_sync(0xffffffffu, at, i);
+        float4* to = reinterpret_cast<float4*>(sh.rows[warp * 16 + i]) + lane;
         if (lane < HD / 4) {
-          if (r < nq)
-            cp_async16(to, reinterpret_cast<const float4*>(p.q + sh.row_at[r]) + lane);
+          if (warp * 16 + i < nq)
+            cp_async16(to, reinterpret_cast<const float4*>(p.q + from) + lane);
           else
             *to = make_float4(0.f, 0.f, 0.f, 0.f);
         }
@@ -467,29 +471,34 @@ __global__ void __launch_bounds__(kTileThreads, 1) paged_tile_kernel(const Paged
       cp_async_commit();
       cp_async_wait<0>();
       asm volatile("bar.sync 1, 256;\n" ::: "memory");
-      const float4* mine = reinterpret_cast<const float4*>(sh.rows[row]);
+      float4 x[HD / 8];
       float top = 0.f, sum = 0.f;
-#pragma unroll 4
-      for (int i = 0; i < HD / 4; ++i) {
-        const float4 x = mine[i];
-        top = max3(top, max3(fabsf(x.x), fabsf(x.y), fabsf(x.z)), fabsf(x.w));
-        sum += (x.x + x.y) + (x.z + x.w);
+#pragma unroll
+      for (int i = 0; i < HD / 8; ++i) {
+        x[i] = reinterpret_cast<const float4*>(sh.rows[row])[half * (HD / 8) + i];
+        top = max3(top, max3(fabsf(x[i].x), fabsf(x[i].y), fabsf(x[i].z)), fabsf(x[i].w));
+        sum += (x[i].x + x[i].y) + (x[i].z + x[i].w);
       }
+      sh.top[0][half][row] = top;
+      sh.top[1][half][row] = sum;
+      asm volatile("bar.sync %0, 64;\n" ::"r"(2 + quad) : "memory");
+      top = fmaxf(top, sh.top[0][half ^ 1][row]);
+      sum = sh.top[1][0][row] + sh.top[1][1][row];
+      asm volatile("bar.sync %0, 64;\n" ::"r"(2 + quad) : "memory");  // read before the tiles' maxima take the place
       const int e = min(max(exponent_of(top), -100), 126);
       const float up = p.scale < 0.f ? -pow2i(13 - e) : pow2i(13 - e);
-#pragma unroll 1
-      for (int i = 0; i < HD / 32; ++i) {
-        uint32_t v[16];
 #pragma unroll
-        for (int k = 0; k < 8; ++k) {
-          const float4 x = mine[i * 8 + k];
-          uint32_t h0, l0, h1, l1;
-          split2(x.x * up, x.y * up, h0, l0);
-          split2(x.z * up, x.w * up, h1, l1);
-          v[2 * k] = half == 0 ? h0 : l0;
-          v[2 * k + 1] = half == 0 ? h1 : l1;
+      for (int i = 0; i < HD / 32; ++i) {
+        uint32_t h[8], l[8];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const float4& y = x[i * 4 + k];
+          split2(y.x * up, y.y * up, h[2 * k], l[2 * k]);
+          split2(y.z * up, y.w * up, h[2 * k + 1], l[2 * k + 1]);
         }
-        tc_st16(tmem + TileTmem<HD>::kQ + lanes + half * (HD / 2) + i * 16, v);
+        const uint32_t to = tmem + TileTmem<HD>::kQ + lanes + half * (HD / 4) + i * 8;
+        tc_st8(to, h);
+        tc_st8(to + HD / 2, l);
       }
       hq = 0.5f * up * sum;
       fq = fabsf(p.scale) * kLog2e * pow2i(e - 13);
@@ -508,14 +517,14 @@ __global__ void __launch_bounds__(kTileThreads, 1) paged_tile_kernel(const Paged
         if (lane == 0) mbar_arrive(&sh.p_full[j % kScoreTiles]);
         continue;
       }
-      ok = ok && mbar_wait(&sh.scales[j & 3], static_cast<uint32_t>(j >> 2) & 1u) &&
-           mbar_wait(&sh.s_full[j % kScoreTiles], static_cast<uint32_t>(j / kScoreTiles) & 1u);
+      ok = ok && mbar_wait(&sh.s_full[j % kScoreTiles], static_cast<uint32_t>(j / kScoreTiles) & 1u);
       __syncwarp();
       tc_after();
       const uint32_t scol = tmem + TileTmem<HD>::kS + (j % kScoreTiles) * kTileK + lanes + half * kHalf;
       uint32_t u[kHalf];
       tc_ld32(scol, u);
       tc_ld32(scol + 32, u + 32);
+      ok = ok && mbar_wait(&sh.scales[j & 3], static_cast<uint32_t>(j >> 2) & 1u);
       const int t0 = tile_pos(j);
       // Scales: K's of this half's four parts, V's exponents of these and of the others.
       const float4 k4 = *reinterpret_cast<const float4*>(&sh.ks[j & 3][half * 4]);
@@ -525,6 +534,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) paged_tile_kernel(const Paged
       const int ve[4] = {v4.x, v4.y, v4.z, v4.w};
       const int low_e = min(min(min(v4.x, v4.y), min(v4.z, v4.w)), min(min(w4.x, w4.y), min(w4.z, w4.w)));
       const int ev = max(max(max(v4.x, v4.y), max(v4.z, v4.w)), max(max(w4.x, w4.y), max(w4.z, w4.w)));
+      __syncwarp();
       tc_wait_ld();
       tc_loaded(u);
       tc_loaded(u + 32);

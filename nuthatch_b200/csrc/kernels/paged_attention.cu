@@ -100,13 +100,15 @@ struct SplitStage {
 constexpr int kSplitStages = 3;
 
 // The values that the warps and the CTAs of a cluster join ([0] holds the CTA's
-// after the join); they take the rings' place once the units are done.
+// after the join); they take the rings' place once the units are done.  Within a
+// query dimension a * (HD / 8) + i, which lane `a` of eight holds, lies at place
+// i * 8 + a, and rows are padded by 8: no two lanes of a store share a bank.
 template <int HD, int NQ>
 struct SplitShared {
   static constexpr int kSplitWarps = kWarpsOf<NQ>;
   union {
     SplitStage<HD> ring[kSplitWarps][kSplitStages];
-    float o[kSplitWarps][NQ][HD];
+    float o[kSplitWarps][NQ][HD + 8];
   };
   float m[kSplitWarps][NQ], l[kSplitWarps][NQ];
   float cm[NQ], cl[NQ];
@@ -308,7 +310,7 @@ __global__ void __launch_bounds__(kWarpsOf<NQ> * 32, NQ == 8 ? 3 : 2) paged_spli
         qa[w][1] = l0;
         qa[w][2] = h1;
         qa[w][3] = l1;
-      } else if (warp == 0) {
+      } else if (w % kSplitWarps == warp) {  // the warps share the words
         uint32_t* hi = reinterpret_cast<uint32_t*>(&sh.qa[w][0][lane]);
         uint32_t* lo = reinterpret_cast<uint32_t*>(&sh.qa[w][1][lane]);
         hi[k] = h0;
@@ -523,8 +525,7 @@ __global__ void __launch_bounds__(kWarpsOf<NQ> * 32, NQ == 8 ? 3 : 2) paged_spli
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
         const float v = kSmall ? o[n][2 * e] + o[n][2 * e + 1] : NQ == 8 ? o[n][e] + o[n][e + 2] : o[n][2 * k + e];
-        const int d = kSmall ? g * VW * 4 + 2 * n + e : (2 * t + e) * VW * 4 + n;
-        sh.o[warp][qk][d] = (v + 0.5f * b[k]) * pow2i(-kWeightShift) * unit;
+        sh.o[warp][qk][kSmall ? (2 * n + e) * 8 + g : n * 8 + 2 * t + e] = (v + 0.5f * b[k]) * pow2i(-kWeightShift) * unit;
       }
   }
   __syncthreads();
@@ -553,14 +554,14 @@ __global__ void __launch_bounds__(kWarpsOf<NQ> * 32, NQ == 8 ? 3 : 2) paged_spli
     __syncthreads();
   const int per = (nq * HD + nrank - 1) / nrank;
   for (int j = rank * per + tid; j < min((rank + 1) * per, nq * HD); j += kSplitThreads) {
-    const int q = j / HD, d = j % HD, qi = q0 + q;
+    const int q = j / HD, d = j % HD, qi = q0 + q, place = d % (HD / 8) * 8 + d / (HD / 8);
     float top = -INFINITY, sum = 0.f, v = 0.f;
     for (int r = 0; r < nrank; ++r) top = fmaxf(top, cluster.map_shared_rank(sh.cm, r)[q]);
     for (int r = 0; r < nrank; ++r) {
       const float mr = cluster.map_shared_rank(sh.cm, r)[q];
       const float a = mr == -INFINITY ? 0.f : exp2_fast(mr - top);
       sum += a * cluster.map_shared_rank(sh.cl, r)[q];
-      v += a * cluster.map_shared_rank(&sh.o[0][0][0], r)[j];
+      v += a * cluster.map_shared_rank(&sh.o[0][q][0], r)[place];
     }
     const int row = sq.r0 + qi / p.group, head = kh * p.group + qi % p.group;
     p.out[(static_cast<int64_t>(row) * p.n_head + head) * HD + d] = sum == 0.f ? 0.f : v / sum;
@@ -579,8 +580,10 @@ int launch_split(const PagedAttnArgs& p, int groups, int ranks, cudaStream_t s) 
                         dim3(kWarpsOf<NQ> * 32), ranks, smem, s, p);
 }
 
-// CTAs of a (sequence, KV head, query group): one, unless the groups alone leave SMs empty.  (More are not free: each
-// forms the query's operand and joins what it has; 16 sequences' 20 queries to 6001 positions take 88 us with 4, 112 with 8.)
+// CTAs of a (sequence, KV head, query group): one, unless the groups alone leave less than eight warps to an SM.  More
+// are not free (each forms the query's operand and joins what it has), so a warp keeps a unit, and a cluster
+// larger than the portable eight, which is slow to start, has more: one sequence's 8,000 positions of 16 heads take
+// 17.6 us with 8 CTAs a head and 22.6 with 16, 131,001 positions 150 and 133.
 template <int HD, int NQ>
 int launch_group(const PagedAttnArgs& p, int groups, cudaStream_t s) {
   if (static_cast<int64_t>(p.kv.n_kv) * groups > 65535) return NH_E_ARG;
@@ -588,7 +591,9 @@ int launch_group(const PagedAttnArgs& p, int groups, cudaStream_t s) {
   const int64_t items = static_cast<int64_t>(p.rows.n_seq) * p.kv.n_kv * groups;
   const int64_t units = static_cast<int64_t>(p.rows.max_blocks) * p.kv.page / kUnit;
   int ranks = 1;
-  while (ranks < 16 && items * ranks * kWarps < 16 * device_sm_count() && units > 2 * kWarps * ranks) ranks *= 2;
+  while (ranks < 16 && items * ranks * kWarps < 8 * device_sm_count() &&
+         units >= (ranks < 8 ? 1 : 16) * kWarps * 2 * ranks)
+    ranks *= 2;
   return launch_split<HD, NQ>(p, groups, ranks, s);
 }
 

@@ -254,10 +254,129 @@ def test_attention_prompt_rows(gpu, n_head, n_kv, hd, page, window, sinks):
     _attend_case(n, p0, n_head, n_kv, hd, page, window, sinks, 13 * n_head + page + window)
 
 
-@pytest.mark.parametrize("n,p0", [([1], [5000]), ([9], [9000]), ([700], [1500])])
+@pytest.mark.parametrize("n,p0", [([1], [5000]), ([9], [9000]), ([700], [1500]), ([40], [5000])])
 def test_attention_long_and_sharp(gpu, n, p0):
     """Long caches with scores far apart (the running maximum moves often)."""
     _attend_case(n, p0, 8, 4, 64, 32, 0, 0, 21, sharp=40.0)
+
+
+def test_attention_zero_queries_and_factors(gpu):
+    """A factor of zero, a negative one and queries of zeros: weights by the formula (equal ones, or turned round), hidden
+    positions hidden."""
+    import torch
+
+    n_head, n_kv, hd, page, total = 4, 2, 64, 16, 200
+    for rows_n, window in ((1, 0), (3, 50), (60, 50), (130, 0)):
+        rng, table, cache, dev = _setup([rows_n], [total - rows_n], n_head, n_kv, hd, page, 8)
+        rows, keep = dev.rows([rows_n], [total - rows_n])
+        k, v = cache.values(0, table[0], total), cache.values(1, table[0], total)
+        for scale, size_q in ((0.0, 1.0), (-0.2, 1.0), (0.1, 0.0), (0.125, 1e-36), (1e-3, 1e3)):
+            q = (rng.standard_normal((rows_n, n_head, hd)) * size_q).astype(np.float32)
+            out = torch.full((rows_n, n_head * hd), 7.0, device="cuda")
+            qd = _cuda(q.reshape(rows_n, -1))
+            assert lib().nh_paged_attention(C.byref(dev.kv), C.byref(rows), P(qd), n_head, scale, window, 2, P(out),
+                                            _stream()) == 0
+            want, size = pm.attention(q, k, v, total - rows_n, scale, window, 2)
+            bound = pm.attention_bound(size, hd, total, np.abs(v).max())
+            err = np.abs(out.cpu().numpy().reshape(want.shape) - want).max()
+            assert err <= bound, (rows_n, window, scale, size_q, err, bound)
+
+
+def test_attention_not_finite_queries_stay_apart(gpu):
+    """A query that holds a NaN or an infinity gives no number in its own row and leaves the others as they are."""
+    import torch
+
+    n_head, n_kv, hd, page = 4, 2, 64, 16
+    for rows_n in (2, 5, 100):
+        total = rows_n + 150
+        rng, table, cache, dev = _setup([rows_n], [150], n_head, n_kv, hd, page, 18)
+        rows, keep = dev.rows([rows_n], [150])
+        q = rng.standard_normal((rows_n, n_head * hd)).astype(np.float32)
+        outs = []
+        for bad in (False, True):
+            if bad:
+                q[1, hd + 5] = np.nan   # row 1, head 1
+                q[0, 3 * hd + 1] = np.inf  # row 0, head 3
+            out = torch.full((rows_n, n_head * hd), 7.0, device="cuda")
+            qd = _cuda(q)
+            assert lib().nh_paged_attention(C.byref(dev.kv), C.byref(rows), P(qd), n_head, 0.125, 0, 0, P(out),
+                                            _stream()) == 0
+            outs.append(out.cpu().numpy().reshape(rows_n, n_head, hd))
+        same = np.ones((rows_n, n_head), bool)
+        same[1, 1] = same[0, 3] = False
+        assert np.array_equal(outs[0][same], outs[1][same])
+        assert np.isnan(outs[1][1, 1]).all() and np.isnan(outs[1][0, 3]).all()
+
+
+def test_attention_far_pages(gpu):
+    """Pages beyond 2^31 bytes of the pool, for every form."""
+    import torch
+
+    n_head, n_kv, hd, page = 16, 16, 128, 128
+    total = 300
+    pages = 10000  # 2.6 GB of codes, keys and values apart
+    codes = [torch.empty(pages, n_kv, page, hd, dtype=torch.uint8, device="cuda") for _ in range(2)]
+    scales = [torch.empty(pages, n_kv, device="cuda") for _ in range(2)]
+    rng = np.random.default_rng(6)
+    small = pm.Cache(3, n_kv, page, hd, rng)
+    order = [9999, 8700, 9100]
+    for w in range(2):
+        codes[w][order] = _cuda(small.codes[w])
+        scales[w][order] = _cuda(small.scales[w])
+    dev = pm.Device(small, np.array([order]))
+    dev.kv = pm.NhPagedKv(codes[0].data_ptr(), codes[1].data_ptr(), scales[0].data_ptr(), scales[1].data_ptr(), pages, page,
+                          n_kv, hd)
+    k, v = small.values(0, [0, 1, 2], total), small.values(1, [0, 1, 2], total)
+    for n in (1, 3, 6, 9, 50):
+        q = rng.standard_normal((n, n_head, hd)).astype(np.float32)
+        rows, keep = dev.rows([n], [total - n])
+        out = torch.empty(n, n_head * hd, device="cuda")
+        qd = _cuda(q.reshape(n, -1))
+        assert lib().nh_paged_attention(C.byref(dev.kv), C.byref(rows), P(qd), n_head, 0.088, 0, 0, P(out), _stream()) == 0
+        want, size = pm.attention(q, k, v, total - n, 0.088, 0, 0)
+        bound = pm.attention_bound(size, hd, total, np.abs(v).max())
+        assert np.abs(out.cpu().numpy().reshape(want.shape) - want).max() <= bound
+    # an append and a read there
+    x = [_cuda(rng.standard_normal((2, n_kv * hd)).astype(np.float32)) for _ in range(2)]
+    cs = _cuda(pm.rope_table(hd, 400))
+    rows, keep = dev.rows([2], [total])
+    assert lib().nh_paged_append(C.byref(dev.kv), C.byref(rows), None, 0, P(x[0]), n_kv * hd, P(x[1]), n_kv * hd, None, None,
+                                 EPS, n_head, P(cs), 400, None, _stream()) == 0
+    ko, vo = (torch.empty(2, n_kv * hd, device="cuda") for _ in range(2))
+    assert lib().nh_paged_read(C.byref(dev.kv), C.byref(rows), F32, P(ko), P(vo), _stream()) == 0
+    sc = scales[1][order[2]].repeat_interleave(hd)
+    assert (vo - x[1]).abs().le(sc / 2).all()
+    assert int(dev.err.item()) == 0
+
+
+def test_two_streams_at_once(gpu):
+    """Calls on two streams over caches of their own, with nothing shared, give what they give alone."""
+    import torch
+
+    cases = []
+    for seed, n, p0 in ((1, [1] * 6, [700, 20, 300, 5, 90, 411]), (2, [200, 1, 90], [60, 500, 0])):
+        rng, table, cache, dev = _setup(n, p0, 8, 4, 128, 32, seed)
+        q = _cuda(rng.standard_normal((sum(n), 8 * 128)).astype(np.float32))
+        rows, keep = dev.rows(n, p0)
+        cases.append((dev, rows, keep, q))
+    streams = [torch.cuda.Stream() for _ in cases]
+
+    def call(c, s):
+        dev, rows, keep, q = c
+        with torch.cuda.stream(s):
+            out = torch.empty_like(q)
+            assert lib().nh_paged_attention(C.byref(dev.kv), C.byref(rows), P(q), 8, 0.09, 0, 0, P(out), _stream()) == 0
+        return out
+
+    alone = []
+    for c, s in zip(cases, streams):
+        s.wait_stream(torch.cuda.default_stream())
+        alone.append(call(c, s))
+        torch.cuda.synchronize()
+    for _ in range(5):
+        got = [call(c, s) for c, s in zip(cases, streams)]
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(got, alone))
 
 
 def test_attention_scales_far_apart(gpu):

@@ -475,8 +475,9 @@ typedef struct NhPagedRows {
 
 /* nh_prefill_qk for a paged cache: QK-norm over the full q and k width (with
  * q_norm and k_norm both null: none), NEOX RoPE at each row's position, the
- * rotated q into qr [n_rows][n_head*head_dim], and the rotated K and raw V rows
- * coded into the cache.  Row r of q, k and v starts r * its stride floats in;
+ * rotated q into qr [n_rows][n_head*head_dim] (nh_prefill_qk's bits), and the
+ * rotated K (worked out in 64 bits and rounded to f32 once) and raw V rows coded
+ * into the cache.  Row r of q, k and v starts r * its stride floats in;
  * rope_cs is nh_rope_table's table of rope_len positions (a sequence past it
  * counts as out of bounds).  q and qr may both be null.  A K or V value that
  * is not finite is coded as the nearest end of the range (a NaN as its middle),

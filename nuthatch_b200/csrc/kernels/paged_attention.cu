@@ -88,6 +88,15 @@ __device__ __forceinline__ void copy4(uint32_t smem, const void* gmem) {
   asm volatile("cp.async.ca.shared.global [%0], [%1], 4;\n" ::"r"(smem), "l"(gmem) : "memory");
 }
 
+__device__ __forceinline__ void add_to(float (&o)[4], const float (&d)[4]) {
+  const float2 a = add2(make_float2(o[0], o[1]), make_float2(d[0], d[1]));
+  const float2 b = add2(make_float2(o[2], o[3]), make_float2(d[2], d[3]));
+  o[0] = a.x;
+  o[1] = a.y;
+  o[2] = b.x;
+  o[3] = b.y;
+}
+
 // One unit of a warp's ring.  Rows of V are padded so that the four rows that a
 // quarter of a warp reads at once lie in different banks; rows of K need that
 // at 128 bytes only, where odd rows swap their halves.
@@ -485,18 +494,26 @@ __global__ void __launch_bounds__(kWarpsOf<NQ> * 32, NQ == 8 ? 3 : 2) paged_spli
       const uint32_t b01 = __byte_perm(vw[2][w], vw[3][w], 0x5140), b23 = __byte_perm(vw[2][w], vw[3][w], 0x7362);
       const uint32_t va[4] = {codes_lo(a01), codes_hi(a01), codes_lo(a23), codes_hi(a23)};
       const uint32_t vb[4] = {codes_lo(b01), codes_hi(b01), codes_lo(b23), codes_hi(b23)};
+      // A unit's products start from zero and join the sums by rounded additions: the tensor cores' own additions cut
+      // off, which over thousands of units would pull every sum towards zero.
       if constexpr (kSmall) {
 #pragma unroll
-        for (int e = 0; e < 2; ++e) mma_f16(o[2 * w + e], va[2 * e], va[2 * e + 1], vb[2 * e], vb[2 * e + 1], b0, b1);
+        for (int e = 0; e < 2; ++e) {
+          float d[4] = {0.f, 0.f, 0.f, 0.f};
+          mma_f16(d, va[2 * e], va[2 * e + 1], vb[2 * e], vb[2 * e + 1], b0, b1);
+          add_to(o[2 * w + e], d);
+        }
       } else {
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
+          float d[4] = {0.f, 0.f, 0.f, 0.f};
           if constexpr (NQ == 8) {
-            mma_f16(o[4 * w + e], hi[0][0], lo[0][0], hi[0][1], lo[0][1], va[e], vb[e]);
+            mma_f16(d, hi[0][0], lo[0][0], hi[0][1], lo[0][1], va[e], vb[e]);
           } else {
-            mma_f16(o[4 * w + e], hi[0][0], hi[1][0], hi[0][1], hi[1][1], va[e], vb[e]);
-            mma_f16(o[4 * w + e], lo[0][0], lo[1][0], lo[0][1], lo[1][1], va[e], vb[e]);
+            mma_f16(d, hi[0][0], hi[1][0], hi[0][1], hi[1][1], va[e], vb[e]);
+            mma_f16(d, lo[0][0], lo[1][0], lo[0][1], lo[1][1], va[e], vb[e]);
           }
+          add_to(o[4 * w + e], d);
         }
       }
     }

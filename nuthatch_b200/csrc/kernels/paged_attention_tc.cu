@@ -20,6 +20,9 @@
 // (Unswizzled operands are read at half the rate: with Q in shared memory too, a
 // 16-wide step of the scores took 138 cycles for 64, and the softmax warps'
 // own accesses waited.)
+// The tensor cores' own additions cut off, which over a long sequence pulls every
+// sum towards zero (9e-6 of it at 4,096 positions): the sums of every few tiles
+// leave tensor memory and are added up in shared memory, rounded.
 // All waits are bounded; an expired one records NH_E_TIMEOUT.
 #include <cooperative_groups.h>
 
@@ -42,6 +45,7 @@ constexpr float kLeast = 1.17549435e-38f;  // factor of the scores at least: a h
 constexpr int kHidden = -1000;     // V's exponent where no position is seen
 constexpr int kHalfBytes = kTileK * 128;  // 64 dimensions of an operand tile
 constexpr int kTileShift = 7;   // weights are 2^7 times [0, 2^8]
+constexpr int kFlush = 2;    // tiles whose products are added up in tensor memory
 constexpr float kGrow = 8.f;    // the maximum in use lags the true one by at most 2^8
 
 constexpr uint32_t kTmemCols = 512;
@@ -165,24 +169,6 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
   asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
   return d;
 }
-// Two f32 operations in one instruction, each rounded as by itself.
-__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
-  float2 d;
-  asm("{\n .reg .b64 x, y, z;\n mov.b64 x, {%2, %3};\n mov.b64 y, {%4, %5};\n mov.b64 z, {%6, %7};\n"
-      " fma.rn.f32x2 x, x, y, z;\n mov.b64 {%0, %1}, x;\n}\n"
-      : "=f"(d.x), "=f"(d.y)
-      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
-  return d;
-}
-__device__ __forceinline__ float2 add2(float2 a, float2 b) {
-  float2 d;
-  asm("{\n .reg .b64 x, y;\n mov.b64 x, {%2, %3};\n mov.b64 y, {%4, %5};\n add.rn.f32x2 x, x, y;\n"
-      " mov.b64 {%0, %1}, x;\n}\n"
-      : "=f"(d.x), "=f"(d.y)
-      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
-  return d;
-}
-
 // Tiles of a sequence in this form.
 __device__ __forceinline__ int tiles_of(const PagedAttnArgs& p, const SeqRows& r) {
   const int64_t n_q = static_cast<int64_t>(r.n) * p.group;
@@ -418,7 +404,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) paged_tile_kernel(const Paged
         if (one) {
 #pragma unroll
           for (int k = 0; k < kTileK / 16; ++k)
-            mma_ts<idesc(HD, true)>(oa, a + (k >> 1) * 32 + (k & 1) * 8, b + k * kStepV, k > 0 || j > 0 ? 1u : 0u);
+            mma_ts<idesc(HD, true)>(oa, a + (k >> 1) * 32 + (k & 1) * 8, b + k * kStepV, k > 0 || j % kFlush > 0 ? 1u : 0u);
 #pragma unroll
           for (int k = 0; k < kTileK / 16; ++k)
             mma_ts<idesc(HD, true)>(oa, a + (k >> 1) * 32 + 16 + (k & 1) * 8, b + k * kStepV, 1u);
@@ -443,6 +429,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) paged_tile_kernel(const Paged
     asm volatile("setmaxnreg.inc.sync.aligned.u32 144;\n");
     float row_m = -INFINITY, row_l = 0.f, row_b = 0.f;  // the row's maximum in use, sum, sum in units of V
     int eref = -200;                                    // O is in units of 2^(eref - kTileShift)
+    float pend = 1.f;  // what the sums in shared memory are still to be scaled by
     const int half = warp >> 2, quad = warp & 3, row = quad * 32 + lane;
     const uint32_t lanes = static_cast<uint32_t>(quad * 32) << 16;
     const int pos = row < nq ? sq.p0 + (q0 + row) / p.group : -1;
@@ -507,6 +494,24 @@ __global__ void __launch_bounds__(kTileThreads, 1) paged_tile_kernel(const Paged
       __syncwarp();
       if (lane == 0) mbar_arrive(&sh.q_full);
     }
+    // This lane's half of the row: sums in shared memory (when `more`) times f, plus those in tensor memory times g.
+    auto add_sums = [&](bool more, float f, float g) {
+#pragma unroll 1
+      for (int i = half * (HD / 32); i < (half + 1) * (HD / 32); ++i) {
+        uint32_t o[16];
+        tc_ld16(tmem + TileTmem<HD>::kO + lanes + i * 16, o);
+        tc_wait_ld();
+        tc_loaded16(o);
+        float4* to = reinterpret_cast<float4*>(&sh.rows[row][i * 16]);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+          if (more) v = to[k];
+          to[k] = make_float4(fmaf(v.x, f, __uint_as_float(o[4 * k]) * g), fmaf(v.y, f, __uint_as_float(o[4 * k + 1]) * g),
+                              fmaf(v.z, f, __uint_as_float(o[4 * k + 2]) * g), fmaf(v.w, f, __uint_as_float(o[4 * k + 3]) * g));
+        }
+      }
+    };
     // No softmax warp leaves the loop early, so that the pairs' barriers stay matched: after an expired wait it runs on
     // without waiting.
     for (int j = 0; j < n; ++j) {
@@ -568,9 +573,10 @@ __global__ void __launch_bounds__(kTileThreads, 1) paged_tile_kernel(const Paged
       top = fmaxf(top, sh.top[j & 1][half ^ 1][row]);
       // The maximum in use follows the true one only when that is 2^8 above it; O follows then, and when V's scale grows.
       const bool grow = top > (row_m == -INFINITY ? row_m : row_m + kGrow);
+      const bool flush = j > 0 && j % kFlush == 0;
+      float alpha = 1.f;
       if (__any_sync(0xffffffffu, grow) || ev > eref) {
         const int en = max(eref, ev);
-        float alpha = 1.f;
         if (grow) {
           alpha = row_m == -INFINITY ? 0.f : exp2_fast(row_m - top);
           row_m = top;
@@ -579,7 +585,8 @@ __global__ void __launch_bounds__(kTileThreads, 1) paged_tile_kernel(const Paged
         alpha *= pow2i(max(eref - en, -200));
         row_b *= alpha;
         eref = en;
-        if (j > 0) {
+        if (j > 0 && !flush) {
+          pend *= alpha;
           ok = ok && products_done(j - 1);
           __syncwarp();
           tc_after();
@@ -635,6 +642,14 @@ __global__ void __launch_bounds__(kTileThreads, 1) paged_tile_kernel(const Paged
         }
         tc_st32(scol + c * 32, w);
       }
+      if (flush) {
+        // The tiles' sums so far, in this tile's units; its own products start from zero.
+        ok = ok && products_done(j - 1);
+        __syncwarp();
+        tc_after();
+        add_sums(j > kFlush, pend * alpha, alpha);
+        pend = 1.f;
+      }
       tc_wait_st();
       tc_before();
       __syncwarp();
@@ -651,22 +666,13 @@ __global__ void __launch_bounds__(kTileThreads, 1) paged_tile_kernel(const Paged
     asm volatile("bar.sync 1, 256;\n" ::: "memory");
     const float b = 0.5f * (sh.b[0][row] + sh.b[1][row]), unit = pow2i(max(eref, -126));
     const float l = sh.l[0][row] + sh.l[1][row], inv = nrank > 1 ? 1.f : l == 0.f ? 0.f : 1.f / l;
-#pragma unroll 1
-    for (int i = half * (HD / 32); i < (half + 1) * (HD / 32); ++i) {
-      uint32_t o[16];
-      if (n > 0) {
-        tc_ld16(tmem + TileTmem<HD>::kO + lanes + i * 16, o);
-        tc_wait_ld();
-        tc_loaded16(o);
-      }
-#pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        float v[4];
-#pragma unroll
-        for (int e = 0; e < 4; ++e)
-          v[e] = n > 0 ? (__uint_as_float(o[4 * k + e]) + b) * pow2i(-kTileShift) * unit * inv : 0.f;
-        *reinterpret_cast<float4*>(&sh.rows[row][i * 16 + k * 4]) = make_float4(v[0], v[1], v[2], v[3]);
-      }
+    if (n > 0 && !idle) add_sums(n > kFlush, pend, 1.f);
+#pragma unroll 4
+    for (int i = half * (HD / 8); i < (half + 1) * (HD / 8); ++i) {
+      float4& v = reinterpret_cast<float4*>(sh.rows[row])[i];
+      const float4 y = n > 0 ? v : make_float4(0.f, 0.f, 0.f, 0.f);
+      v = make_float4((y.x + b) * pow2i(-kTileShift) * unit * inv, (y.y + b) * pow2i(-kTileShift) * unit * inv,
+                      (y.z + b) * pow2i(-kTileShift) * unit * inv, (y.w + b) * pow2i(-kTileShift) * unit * inv);
     }
     tc_before();
   }

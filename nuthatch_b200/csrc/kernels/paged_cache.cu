@@ -8,7 +8,9 @@
 // columns for every row of the page and writes the sums to all CTAs (distributed
 // shared memory); from there each works on whole (page, head) pairs alone: a
 // few warps a head, four rows of K and V a warp held in registers from the load
-// (issued before the norm's barrier) to the codes.  Per row the arithmetic is nh_prefill_qk's.
+// (issued before the norm's barrier) to the codes.  q's arithmetic is
+// nh_prefill_qk's; K's norm and rotation are in 64 bits, rounded to f32 once, so
+// that a value next to a code's border falls on the side where it belongs.
 //
 // What bounds it: one row a sequence, the chain of dependent loads and the
 // cluster's barrier; prompts, the bytes (q and K are read a second time, out of
@@ -72,7 +74,8 @@ struct AppendShape {
 template <int PAGE>
 struct AppendShared {
   double sums[kMaxRanks][PAGE][2];              // every CTA's sums of squares of each row's q, k
-  float scq[PAGE], sck[PAGE];                   // each row's RMSNorm factors
+  double sck[PAGE];                             // each row's RMSNorm factor of k, of q
+  float scq[PAGE];
   uint32_t top[2][AppendShape<PAGE>::kHeads][2];  // bits of the largest magnitude of a head's K, V (two rounds)
 };
 
@@ -84,6 +87,21 @@ __device__ __forceinline__ double squares(const float* x, int n4, int lane) {
     const float4 v = __ldg(reinterpret_cast<const float4*>(x) + i);
     s += (static_cast<double>(__fmul_rn(v.x, v.x)) + static_cast<double>(__fmul_rn(v.y, v.y))) +
          (static_cast<double>(__fmul_rn(v.z, v.z)) + static_cast<double>(__fmul_rn(v.w, v.w)));
+  }
+  return s;
+}
+
+// The same with the products in 64 bits.
+__device__ __forceinline__ double squares64(const float* x, int n4, int lane) {
+  double s = 0.0;
+#pragma unroll 4
+  for (int i = lane; i < n4; i += 32) {
+    const float4 v = __ldg(reinterpret_cast<const float4*>(x) + i);
+    const double a = v.x, b = v.y, c = v.z, d = v.w;
+    s = fma(a, a, s);
+    s = fma(b, b, s);
+    s = fma(c, c, s);
+    s = fma(d, d, s);
   }
   return s;
 }
@@ -121,6 +139,21 @@ __device__ __forceinline__ void turn(Pair<N>& x, bool norm, float sc, const Pair
     }
     x.lo[e] = __fsub_rn(__fmul_rn(x0, cs[2 * e]), __fmul_rn(x1, cs[2 * e + 1]));
     x.hi[e] = __fadd_rn(__fmul_rn(x0, cs[2 * e + 1]), __fmul_rn(x1, cs[2 * e]));
+  }
+}
+// The same in 64 bits, rounded once.
+template <int N>
+__device__ __forceinline__ void turn64(Pair<N>& x, bool norm, double sc, const Pair<N>& w, const float (&cs)[2 * N]) {
+#pragma unroll
+  for (int e = 0; e < N; ++e) {
+    double x0 = x.lo[e], x1 = x.hi[e];
+    if (norm) {
+      x0 *= sc * static_cast<double>(w.lo[e]);
+      x1 *= sc * static_cast<double>(w.hi[e]);
+    }
+    const double c = cs[2 * e], s = cs[2 * e + 1];
+    x.lo[e] = static_cast<float>(fma(x0, c, -(x1 * s)));
+    x.hi[e] = static_cast<float>(fma(x0, s, x1 * c));
   }
 }
 template <int N>
@@ -224,7 +257,7 @@ __global__ void __launch_bounds__(AppendShape<PAGE>::kThreads, 1024 / AppendShap
     bool started = false;
     for (int t = warp; t < nt; t += S::kWarps) {
       double a = has_q ? squares(q0 + t * qs + qh0 * HD, (qh1 - qh0) * (HD / 4), lane) : 0.0;
-      double c = squares(k0 + t * ks + kh0 * HD, (kh1 - kh0) * (HD / 4), lane);
+      double c = squares64(k0 + t * ks + kh0 * HD, (kh1 - kh0) * (HD / 4), lane);
       a = warp_sum_d(a);
       c = warp_sum_d(c);
       if (!started) {
@@ -246,7 +279,7 @@ __global__ void __launch_bounds__(AppendShape<PAGE>::kThreads, 1024 / AppendShap
         c += sh.sums[r][t][1];
       }
       sh.scq[t] = __fdiv_rn(1.0f, __fsqrt_rn(__fadd_rn(static_cast<float>(div_count(a, dq)), p.eps)));
-      sh.sck[t] = __fdiv_rn(1.0f, __fsqrt_rn(__fadd_rn(static_cast<float>(div_count(c, dkv)), p.eps)));
+      sh.sck[t] = 1.0 / sqrt(c / dkv + static_cast<double>(p.eps));
     }
   }
   __syncthreads();
@@ -299,7 +332,7 @@ __global__ void __launch_bounds__(AppendShape<PAGE>::kThreads, 1024 / AppendShap
           if (t < nt) {
             float cs[2 * N];
             load_cs<N>(cs0 + t * HD, i, cs);
-            turn<N>(k[r], norm, norm ? sh.sck[t] : 1.f, w, cs);
+            turn64<N>(k[r], norm, norm ? sh.sck[t] : 1.0, w, cs);
             mk = top_of<N>(k[r], mk);
             mv = top_of<N>(v[r], mv);
           }

@@ -1,7 +1,7 @@
 """The paged 8-bit K/V cache and the draft check in numpy, for the tests: the
-formulas of nh_kernels.h in 64 bits (the coded rows in the kernels' f32 steps,
-each a correctly rounded IEEE operation, so that codes can be compared bit for
-bit)."""
+formulas of nh_kernels.h in 64 bits (the rotated q in the kernels' f32 steps,
+each a correctly rounded IEEE operation; K's rows rounded to f32 once, so that
+codes can be compared bit for bit)."""
 from __future__ import annotations
 
 import ctypes as C
@@ -32,6 +32,17 @@ def rotated_rows(x: np.ndarray, w, pos: np.ndarray, cs: np.ndarray, heads: int, 
     lo = x[:, :, 0] * c - x[:, :, 1] * s
     hi = x[:, :, 0] * s + x[:, :, 1] * c
     return np.concatenate([lo, hi], -1)  # [n][heads][hd]
+
+
+def rotated_keys(x: np.ndarray, w, pos: np.ndarray, cs: np.ndarray, heads: int, eps: float) -> np.ndarray:
+    """The same in f64, rounded to f32 at the end."""
+    n, hd = x.shape[0], x.shape[1] // heads
+    x = x.astype(np.float64)
+    if w is not None:
+        x = x / np.sqrt((x * x).mean(1, keepdims=True) + np.float64(F(eps))) * w.astype(np.float64)
+    x = x.reshape(n, heads, 2, hd // 2)
+    c, s = (cs[pos][:, None, :, i].astype(np.float64) for i in range(2))
+    return np.concatenate([x[:, :, 0] * c - x[:, :, 1] * s, x[:, :, 0] * s + x[:, :, 1] * c], -1).astype(F)
 
 
 def scale_for(m: float) -> float:

@@ -236,7 +236,7 @@ __global__ void __launch_bounds__(kWarpsOf<NQ> * 32, NQ == 8 ? 3 : 2) paged_spli
   uint32_t qa[NQ == 4 || NQ == 8 ? KS : 1][4], qd[NQ == 2 ? KS : 1];
   int h0 = 0, h1 = 0;            // 2 queries: 255 times the digit sums of this lane's two columns,
   float m0 = 0.f, m1 = 0.f;      // and half of what their digits stand for
-  float fq[QT], hq[QT];
+  float fq[QT], nan_q = 0.f;  // nan_q: 2 queries, see below
   int pos[QT];
 #pragma unroll
   for (int k = 0; k < QT; ++k) {
@@ -260,11 +260,11 @@ __global__ void __launch_bounds__(kWarpsOf<NQ> * 32, NQ == 8 ? 3 : 2) paged_spli
       // Whole numbers of at most 2^22, column g: digit 0 or 1 of query (g / 2) % 2 for g < 4, else 2 (even) or none.  A
       // warp forms its share of the words for all of them.
       const float up = pow2i(21 - e);
-      float off = 0.f;  // a NaN where the query holds a value that is not finite
+      // nan_q: a NaN where the query holds a value that is not finite (which whole numbers do not show).
       const int digit = g < 4 ? g & 1 : 2;
 #pragma unroll
       for (int w = 0; w < KS; ++w) {
-        off += (x[w].x * 0.f + x[w].y * 0.f) + (x[w].z * 0.f + x[w].w * 0.f);
+        nan_q += (x[w].x * 0.f + x[w].y * 0.f) + (x[w].z * 0.f + x[w].w * 0.f);
         if (w % kSplitWarps == warp) {
           const float y[4] = {x[w].x, x[w].y, x[w].z, x[w].w};
           uint32_t word = 0u;
@@ -290,27 +290,25 @@ __global__ void __launch_bounds__(kWarpsOf<NQ> * 32, NQ == 8 ? 3 : 2) paged_spli
       }
       sum += __shfl_xor_sync(0xffffffffu, sum, 1);
       sum += __shfl_xor_sync(0xffffffffu, sum, 2);
-      off += __shfl_xor_sync(0xffffffffu, off, 1);
-      off += __shfl_xor_sync(0xffffffffu, off, 2);
+      nan_q += __shfl_xor_sync(0xffffffffu, nan_q, 1);
+      nan_q += __shfl_xor_sync(0xffffffffu, nan_q, 2);
       // Scores: columns 2 t and 2 t + 1, query t % 2.
       h0 = 255 * __shfl_sync(0xffffffffu, sum, 8 * t);
       h1 = 255 * __shfl_sync(0xffffffffu, sum, 8 * t + 4);
       m0 = t < 2 ? 32768.f : 0.5f;
       m1 = t < 2 ? 128.f : 0.f;
-      hq[k] = __shfl_sync(0xffffffffu, off, 8 * (t & 1));
+      nan_q = __shfl_sync(0xffffffffu, nan_q, 8 * (t & 1));
       fq[k] = __shfl_sync(0xffffffffu, p.scale * kLog2e * pow2i(e - 21), 8 * (t & 1));
       pos[k] = __shfl_sync(0xffffffffu, pos[k], 8 * (t & 1));
       continue;
     }
     // The largest magnitude goes to [2^13, 2^14).
     const float up = pow2i(13 - e);
-    float sum = 0.f;
 #pragma unroll
     for (int w = 0; w < KS; ++w) {
       uint32_t h0, l0, h1, l1;
       split2(x[w].x * up, x[w].y * up, h0, l0);
       split2(x[w].z * up, x[w].w * up, h1, l1);
-      sum += (x[w].x * up + x[w].y * up) + (x[w].z * up + x[w].w * up);
       if constexpr (NQ == 4) {
         qa[w][0] = g & 1 ? l0 : h0;
         qa[w][1] = g & 1 ? l1 : h1;
@@ -328,12 +326,8 @@ __global__ void __launch_bounds__(kWarpsOf<NQ> * 32, NQ == 8 ? 3 : 2) paged_spli
         lo[2 + k] = l1;
       }
     }
-    sum += __shfl_xor_sync(0xffffffffu, sum, 1);
-    sum += __shfl_xor_sync(0xffffffffu, sum, 2);
-    hq[k] = 0.5f * sum;
-    fq[k] = p.scale * kLog2e * pow2i(e - 13);
+    fq[k] = p.scale * kLog2e * pow2i(e - 13 + kCodeShift);
     if constexpr (NQ == 4) {  // scores: query t, whose operand lanes 8 t hold
-      hq[k] = __shfl_sync(0xffffffffu, hq[k], 8 * t);
       fq[k] = __shfl_sync(0xffffffffu, fq[k], 8 * t);
       pos[k] = __shfl_sync(0xffffffffu, pos[k], 8 * t);
     }
@@ -343,13 +337,13 @@ __global__ void __launch_bounds__(kWarpsOf<NQ> * 32, NQ == 8 ? 3 : 2) paged_spli
   float o[ON][4];
 #pragma unroll
   for (int i = 0; i < ON; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
-  float m[QT], l[QT], b[QT];  // running maximum; sum of the weights; sum of the weights in units of the values
+  float m[QT], l[QT];  // running maximum; sum of the weights
 #pragma unroll
   for (int k = 0; k < QT; ++k) {
     m[k] = -INFINITY;
-    l[k] = b[k] = 0.f;
+    l[k] = 0.f;
   }
-  int eref = -200;  // the accumulators are in units of 2^(eref - kWeightShift)
+  int eref = -200;  // the sums are in units of 2^(eref - kWeightShift + kCodeShift)
 
   int st = 0;
   for (int i = i0; i < u1; i += kSplitWarps) {
@@ -413,7 +407,7 @@ __global__ void __launch_bounds__(kWarpsOf<NQ> * 32, NQ == 8 ? 3 : 2) paged_spli
                         : NQ == 4 ? (c[0][2 * e] + c[1][2 * e]) + (c[0][2 * e + 1] + c[1][2 * e + 1])
                         : NQ == 8 ? c[e >> 1][e & 1] + c[e >> 1][(e & 1) + 2]
                                   : c[e >> 1][2 * k + (e & 1)];
-        x[k][e] = (d + hq[k]) * f;
+        x[k][e] = (NQ == 2 ? d + nan_q : d) * f;
       }
       if (!plain) {
 #pragma unroll
@@ -441,7 +435,6 @@ __global__ void __launch_bounds__(kWarpsOf<NQ> * 32, NQ == 8 ? 3 : 2) paged_spli
         const float a = m[k] == -INFINITY ? 0.f : exp2_fast(m[k] - top[k]);
         m[k] = top[k];
         l[k] *= a;
-        b[k] *= a * fe;
 #pragma unroll
         for (int n = 0; n < ON; ++n) {
           if constexpr (NQ <= 8) {
@@ -468,7 +461,6 @@ __global__ void __launch_bounds__(kWarpsOf<NQ> * 32, NQ == 8 ? 3 : 2) paged_spli
         w[e] = exp2_fast(x[k][e] - base);
         l[k] += w[e];
         w[e] *= fw;
-        b[k] += w[e];
       }
       if constexpr (kSmall) {
         // Column g of B: query g / 2's weights at positions 2 t, 2 t + 1 and 8 further, from the lanes that hold them.
@@ -529,7 +521,6 @@ __global__ void __launch_bounds__(kWarpsOf<NQ> * 32, NQ == 8 ? 3 : 2) paged_spli
 #pragma unroll
     for (int e = kSmall ? 4 : 1; e <= (kSmall ? 16 : 2); e <<= 1) {
       l[k] += __shfl_xor_sync(0xffffffffu, l[k], e);
-      b[k] += __shfl_xor_sync(0xffffffffu, b[k], e);
     }
     const int qk = kSmall ? t : g + 8 * k;
     if (kSmall && t >= NQ) continue;  // columns without a query
@@ -542,7 +533,7 @@ __global__ void __launch_bounds__(kWarpsOf<NQ> * 32, NQ == 8 ? 3 : 2) paged_spli
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
         const float v = kSmall ? o[n][2 * e] + o[n][2 * e + 1] : NQ == 8 ? o[n][e] + o[n][e + 2] : o[n][2 * k + e];
-        sh.o[warp][qk][kSmall ? (2 * n + e) * 8 + g : n * 8 + 2 * t + e] = (v + 0.5f * b[k]) * pow2i(-kWeightShift) * unit;
+        sh.o[warp][qk][kSmall ? (2 * n + e) * 8 + g : n * 8 + 2 * t + e] = v * pow2i(kCodeShift - kWeightShift) * unit;
       }
   }
   __syncthreads();

@@ -2,11 +2,10 @@
 // range, exact 8-bit codes as f16 operands and the two-part split of f32
 // factors.
 //
-// Arithmetic.  A code u stands for (c + 1/2) * s with c = u - 128 and s a power
-// of two, so c is exact in f16.  A query row is scaled by a power of two and
+// Arithmetic.  A code u stands for (u - 127.5) * s with s a power of two, and
+// (u - 127.5) * 2^-9 is exact in f16.  A query row is scaled by a power of two and
 // split into two f16 parts (22 bits of it), likewise a softmax weight; both
-// parts' products are exact and the tensor cores add them up in f32.  The half
-// codes come in apart: 1/2 * sum(q) per score, 1/2 * sum(w) per output.
+// parts' products are exact and the tensor cores add them up in f32.
 #pragma once
 
 #include "common.cuh"
@@ -31,10 +30,13 @@ constexpr int kWeightShift = 15;  // a weight in [0, 1] times 2^15 keeps 22 bits
 __device__ __forceinline__ float pow2i(int e) { return e < -126 ? 0.f : __int_as_float((e + 127) << 23); }
 __device__ __forceinline__ int exponent_of(float s) { return ((__float_as_int(s) >> 23) & 255) - 127; }
 
-// Bytes 0, 1 (or 2, 3) of w as two f16 codes c = u - 128: 0x64uu is 1024 + u.
+// Bytes 0, 1 (or 2, 3) of w as (u - 127.5) * 2^-9: the byte alone is the f16
+// u * 2^-24, which one fused step scales and moves, exactly.
+constexpr int kCodeShift = 9;
 __device__ __forceinline__ uint32_t codes_f16(uint32_t w, uint32_t sel) {
-  const uint32_t x = __byte_perm(w, 0x64646464u, sel);
-  const __half2 r = __hsub2(*reinterpret_cast<const __half2*>(&x), __half2half2(__ushort_as_half(0x6480)));
+  const uint32_t x = __byte_perm(w, 0u, sel);
+  const __half2 r = __hfma2(*reinterpret_cast<const __half2*>(&x), __half2half2(__ushort_as_half(0x7800)),   // 2^15
+                            __half2half2(__ushort_as_half(0xB3F8)));                                       // -127.5 * 2^-9
   return *reinterpret_cast<const uint32_t*>(&r);
 }
 __device__ __forceinline__ uint32_t codes_lo(uint32_t w) { return codes_f16(w, 0x4140); }

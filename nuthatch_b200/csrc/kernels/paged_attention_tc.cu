@@ -70,7 +70,7 @@ struct TileShared {
   float top[2][2][kTileQ];  // the halves' maxima of a row (two tiles)
   int64_t row_at[kTileQ];  // where a query's row starts in q and out
   uint64_t full[2][2], empty[2][2], scales[4], q_full, s_full[kScoreTiles], p_full[kScoreTiles], pv_done[kScoreTiles], drained;
-  float m[kTileQ], l[2][kTileQ], b[2][kTileQ];
+  float m[kTileQ], l[2][kTileQ];
   uint32_t tmem;
   int failed;
 };
@@ -427,14 +427,14 @@ __global__ void __launch_bounds__(kTileThreads, 1) paged_tile_kernel(const Paged
   } else {
     // ---------------------------------------------------------------- softmax: a row a lane, half of the positions
     asm volatile("setmaxnreg.inc.sync.aligned.u32 144;\n");
-    float row_m = -INFINITY, row_l = 0.f, row_b = 0.f;  // the row's maximum in use, sum, sum in units of V
-    int eref = -200;                                    // O is in units of 2^(eref - kTileShift)
+    float row_m = -INFINITY, row_l = 0.f;  // the row's maximum in use, sum of its weights
+    int eref = -200;                       // O is in units of 2^(eref - kTileShift + kCodeShift)
     float pend = 1.f;  // what the sums in shared memory are still to be scaled by
     const int half = warp >> 2, quad = warp & 3, row = quad * 32 + lane;
     const uint32_t lanes = static_cast<uint32_t>(quad * 32) << 16;
     const int pos = row < nq ? sq.p0 + (q0 + row) / p.group : -1;
     const bool idle = quad * 32 >= nq;  // no row of this warp is a query
-    float fq, hq;
+    float fq;
     {
       // The rows, read whole; then the two lanes of a row scale half of it each so that the largest magnitude is in
       // [2^13, 2^14), and split it.  A negative factor of the scores changes the query's sign.
@@ -459,18 +459,15 @@ __global__ void __launch_bounds__(kTileThreads, 1) paged_tile_kernel(const Paged
       cp_async_wait<0>();
       asm volatile("bar.sync 1, 256;\n" ::: "memory");
       float4 x[HD / 8];
-      float top = 0.f, sum = 0.f;
+      float top = 0.f;
 #pragma unroll
       for (int i = 0; i < HD / 8; ++i) {
         x[i] = reinterpret_cast<const float4*>(sh.rows[row])[half * (HD / 8) + i];
         top = max3(top, max3(fabsf(x[i].x), fabsf(x[i].y), fabsf(x[i].z)), fabsf(x[i].w));
-        sum += (x[i].x + x[i].y) + (x[i].z + x[i].w);
       }
       sh.top[0][half][row] = top;
-      sh.top[1][half][row] = sum;
       asm volatile("bar.sync %0, 64;\n" ::"r"(2 + quad) : "memory");
       top = fmaxf(top, sh.top[0][half ^ 1][row]);
-      sum = sh.top[1][0][row] + sh.top[1][1][row];
       asm volatile("bar.sync %0, 64;\n" ::"r"(2 + quad) : "memory");  // read before the tiles' maxima take the place
       const int e = min(max(exponent_of(top), -100), 126);
       const float up = p.scale < 0.f ? -pow2i(13 - e) : pow2i(13 - e);
@@ -487,8 +484,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) paged_tile_kernel(const Paged
         tc_st8(to, h);
         tc_st8(to + HD / 2, l);
       }
-      hq = 0.5f * up * sum;
-      fq = fabsf(p.scale) * kLog2e * pow2i(e - 13);
+      fq = fabsf(p.scale) * kLog2e * pow2i(e - 13 + kCodeShift);
       tc_wait_st();
       tc_before();
       __syncwarp();
@@ -566,7 +562,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) paged_tile_kernel(const Paged
         float t = fmaxf(x[b * kSub], x[b * kSub + 1]);
 #pragma unroll
         for (int i = 2; i < kSub; i += 2) t = max3(t, x[b * kSub + i], x[b * kSub + i + 1]);
-        top = fmaxf(top, (t + hq) * fmaxf(fq * ks[b], kLeast));
+        top = fmaxf(top, t * fmaxf(fq * ks[b], kLeast));
       }
       sh.top[j & 1][half][row] = top;
       asm volatile("bar.sync %0, 64;\n" ::"r"(2 + quad) : "memory");  // the other half's warp
@@ -583,7 +579,6 @@ __global__ void __launch_bounds__(kTileThreads, 1) paged_tile_kernel(const Paged
           row_l *= alpha;
         }
         alpha *= pow2i(max(eref - en, -200));
-        row_b *= alpha;
         eref = en;
         if (j > 0 && !flush) {
           pend *= alpha;
@@ -611,7 +606,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) paged_tile_kernel(const Paged
         for (int d = 0; d < 2; ++d) {
           const int b = 2 * c + d, eb = ve[b] - eref + kTileShift;
           const float a = fmaxf(fq * ks[b], kLeast);
-          float off = hq * a - base;
+          float off = -base;
           if (eb < -60) {
             // Hidden, or a scale 2^60 below the largest: the weights count for the sum alone.
             float sum = 0.f;
@@ -638,7 +633,6 @@ __global__ void __launch_bounds__(kTileThreads, 1) paged_tile_kernel(const Paged
           }
           const float sum = sum2.x + sum2.y;
           row_l += sum * pow2i(min(-eb, 60));
-          row_b += sum;
         }
         tc_st32(scol + c * 32, w);
       }
@@ -661,18 +655,17 @@ __global__ void __launch_bounds__(kTileThreads, 1) paged_tile_kernel(const Paged
     __syncwarp();
     tc_after();
     sh.l[half][row] = row_l;
-    sh.b[half][row] = row_b;
     if (half == 0) sh.m[row] = row_m;
     asm volatile("bar.sync 1, 256;\n" ::: "memory");
-    const float b = 0.5f * (sh.b[0][row] + sh.b[1][row]), unit = pow2i(max(eref, -126));
+    const float unit = pow2i(max(eref, -126));
     const float l = sh.l[0][row] + sh.l[1][row], inv = nrank > 1 ? 1.f : l == 0.f ? 0.f : 1.f / l;
     if (n > 0 && !idle) add_sums(n > kFlush, pend, 1.f);
 #pragma unroll 4
     for (int i = half * (HD / 8); i < (half + 1) * (HD / 8); ++i) {
       float4& v = reinterpret_cast<float4*>(sh.rows[row])[i];
       const float4 y = n > 0 ? v : make_float4(0.f, 0.f, 0.f, 0.f);
-      v = make_float4((y.x + b) * pow2i(-kTileShift) * unit * inv, (y.y + b) * pow2i(-kTileShift) * unit * inv,
-                      (y.z + b) * pow2i(-kTileShift) * unit * inv, (y.w + b) * pow2i(-kTileShift) * unit * inv);
+      const float f = pow2i(kCodeShift - kTileShift);
+      v = make_float4(y.x * f * unit * inv, y.y * f * unit * inv, y.z * f * unit * inv, y.w * f * unit * inv);
     }
     tc_before();
   }

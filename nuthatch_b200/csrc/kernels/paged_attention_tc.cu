@@ -45,7 +45,7 @@ constexpr float kLeast = 1.17549435e-38f;  // factor of the scores at least: a h
 constexpr int kHidden = -1000;     // V's exponent where no position is seen
 constexpr int kHalfBytes = kTileK * 128;  // 64 dimensions of an operand tile
 constexpr int kTileShift = 7;   // weights are 2^7 times [0, 2^8]
-constexpr int kFlush = 2;    // tiles whose products are added up in tensor memory
+constexpr int kFlush = 4;    // tiles whose products are added up in tensor memory
 constexpr float kGrow = 8.f;    // the maximum in use lags the true one by at most 2^8
 
 constexpr uint32_t kTmemCols = 512;
@@ -382,8 +382,10 @@ __global__ void __launch_bounds__(kTileThreads, 1) paged_tile_kernel(const Paged
         const uint32_t d = tmem + TileTmem<HD>::kS + (j % kScoreTiles) * kTileK;
         if (one) {
 #pragma unroll
-          for (int k = 0; k < HD / 8; ++k)  // the high parts' steps, then the low ones'
-            mma_ts<idesc(kTileK, false)>(d, qa + k * 8, b + step_k(k % (HD / 16)), k > 0 ? 1u : 0u);
+          for (int k = 0; k < HD / 8; ++k) {  // the low parts' steps first, while the sums they cut are small
+            const int step = k % (HD / 16), part = k < HD / 16 ? HD / 2 : 0;
+            mma_ts<idesc(kTileK, false)>(d, qa + part + step * 8, b + step_k(step), k > 0 ? 1u : 0u);
+          }
           tc_commit(&sh.empty[0][j & 1]);
           tc_commit(&sh.s_full[j % kScoreTiles]);
         }
@@ -403,11 +405,11 @@ __global__ void __launch_bounds__(kTileThreads, 1) paged_tile_kernel(const Paged
         const uint32_t a = tmem + TileTmem<HD>::kS + (j % kScoreTiles) * kTileK;
         if (one) {
 #pragma unroll
-          for (int k = 0; k < kTileK / 16; ++k)
-            mma_ts<idesc(HD, true)>(oa, a + (k >> 1) * 32 + (k & 1) * 8, b + k * kStepV, k > 0 || j % kFlush > 0 ? 1u : 0u);
-#pragma unroll
-          for (int k = 0; k < kTileK / 16; ++k)
-            mma_ts<idesc(HD, true)>(oa, a + (k >> 1) * 32 + 16 + (k & 1) * 8, b + k * kStepV, 1u);
+          for (int k = 0; k < kTileK / 8; ++k) {
+            const int step = k % (kTileK / 16), part = k < kTileK / 16 ? 16 : 0;  // low, high
+            mma_ts<idesc(HD, true)>(oa, a + (step >> 1) * 32 + part + (step & 1) * 8, b + step * kStepV,
+                                    k > 0 || j % kFlush > 0 ? 1u : 0u);
+          }
           tc_commit(&sh.empty[1][j & 1]);
           tc_commit(&sh.pv_done[j % kScoreTiles]);
         }

@@ -482,7 +482,7 @@ typedef struct NhPagedRows {
  * counts as out of bounds).  q and qr may both be null.  A K or V value that
  * is not finite is coded as the nearest end of the range (a NaN as its middle),
  * sets no scale, and records NH_E_ARG in *err.  Pointers are 16-byte aligned, strides
-  * a multiple of 4 and at most 2^23. */
+ * a multiple of 4 and at most 2^23. */
 int nh_paged_append(const NhPagedKv* kv, const NhPagedRows* rows, const float* q, int64_t q_stride, const float* k,
                     int64_t k_stride, const float* v, int64_t v_stride, const float* q_norm, const float* k_norm,
                     float eps, int n_head, const float* rope_cs, int rope_len, float* qr, void* stream);

@@ -255,7 +255,7 @@ __global__ void __launch_bounds__(kWarpsOf<NQ> * 32, NQ == 8 ? 3 : 2) paged_spli
     }
     top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
     top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-    const int e = min(max(exponent_of(top), -100), 126);
+    const int e = min(max(exponent_of(top), -100), 127);
     if constexpr (NQ == 2) {
       // Whole numbers of at most 2^22, column g: digit 0 or 1 of query (g / 2) % 2 for g < 4, else 2 (even) or none.  A
       // warp forms its share of the words for all of them.
@@ -639,7 +639,8 @@ extern "C" int nh_paged_attention(const NhPagedKv* kv, const NhPagedRows* rows, 
   const int rc = paged_args(kv, rows, p.kv, p.rows);
   if (rc != NH_OK) return rc;
   if (qr == nullptr || out == nullptr || !paged_aligned(qr) || !paged_aligned(out) || n_head <= 0 || n_head > 65535 ||
-      n_head % p.kv.n_kv != 0 || window < 0 || n_sink < 0)
+      n_head % p.kv.n_kv != 0 || window < 0 || n_sink < 0 ||
+      static_cast<int64_t>(p.rows.max_rows) * (n_head / p.kv.n_kv) > INT32_MAX)  // queries are counted in 32 bits
     return NH_E_ARG;
   if (p.rows.max_rows == 0) return NH_OK;
   p.q = qr;

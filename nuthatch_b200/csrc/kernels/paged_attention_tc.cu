@@ -184,6 +184,7 @@ __device__ __forceinline__ bool find_tile(const PagedAttnArgs& p, int64_t cap, i
     const int s = s0 + lane;
     SeqRows r{0, 0, 0};
     if (s < p.rows.n_seq) r = seq_rows(p.rows, s, cap);
+    if (r.n < 0 && blockIdx.x == 0) paged_error(p.rows);
     const int mine = tiles_of(p, r);
     int inc = mine;  // tiles of this sequence and the later ones of the 32
 #pragma unroll
@@ -471,7 +472,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) paged_tile_kernel(const Paged
       asm volatile("bar.sync %0, 64;\n" ::"r"(2 + quad) : "memory");
       top = fmaxf(top, sh.top[0][half ^ 1][row]);
       asm volatile("bar.sync %0, 64;\n" ::"r"(2 + quad) : "memory");  // read before the tiles' maxima take the place
-      const int e = min(max(exponent_of(top), -100), 126);
+      const int e = min(max(exponent_of(top), -100), 127);
       const float up = p.scale < 0.f ? -pow2i(13 - e) : pow2i(13 - e);
 #pragma unroll
       for (int i = 0; i < HD / 32; ++i) {

@@ -534,7 +534,7 @@ extern "C" int nh_paged_append(const NhPagedKv* kv, const NhPagedRows* rows, con
   p.q = q;
   p.k = k;
   p.v = v;
-  p.q_stride = q_stride;
+  p.q_stride = q != nullptr ? q_stride : 0;
   p.k_stride = k_stride;
   p.v_stride = v_stride;
   p.q_norm = q_norm;

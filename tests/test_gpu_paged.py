@@ -273,8 +273,8 @@ def test_attention_zero_queries_and_factors(gpu):
         rng, table, cache, dev = _setup([rows_n], [total - rows_n], n_head, n_kv, hd, page, 8)
         rows, keep = dev.rows([rows_n], [total - rows_n])
         k, v = cache.values(0, table[0], total), cache.values(1, table[0], total)
-        for scale, size_q in ((0.0, 1.0), (-0.2, 1.0), (0.1, 0.0), (0.125, 1e-36), (1e-3, 1e3)):
-            q = (rng.standard_normal((rows_n, n_head, hd)) * size_q).astype(np.float32)
+        for scale, size_q in ((0.0, 1.0), (-0.2, 1.0), (0.1, 0.0), (0.125, 1e-36), (1e-3, 1e3), (2.0**-126, 8e37)):
+            q = np.clip(rng.standard_normal((rows_n, n_head, hd)) * size_q, -3.2e38, 3.2e38).astype(np.float32)
             out = torch.full((rows_n, n_head * hd), 7.0, device="cuda")
             qd = _cuda(q.reshape(rows_n, -1))
             assert lib().nh_paged_attention(C.byref(dev.kv), C.byref(rows), P(qd), n_head, scale, window, 2, P(out),
@@ -465,6 +465,13 @@ def test_bad_pages_and_sequences(gpu):
         ko = torch.full((sum(m), dkv), 7.0, device="cuda")
         assert lib().nh_paged_read(C.byref(dev.kv), C.byref(rows), F32, P(ko), None, _stream()) == 0
         assert torch.count_nonzero(ko) == 0
+    # one sequence alone, of many rows, past its pages
+    dev.err.zero_()
+    out = torch.full((R, n_head * hd), 7.0, device="cuda")
+    rows, keep = dev.rows([R], [1 << 20])
+    assert lib().nh_paged_attention(C.byref(dev.kv), C.byref(rows), P(q), n_head, 0.125, 0, 0, P(out), _stream()) == 0
+    torch.cuda.synchronize()
+    assert int(dev.err.item()) == NH_E_ARG and (out == 7.0).all()
     # more rows than the call's bounds say: left alone
     dev.err.zero_()
     out = torch.full((R, n_head * hd), 7.0, device="cuda")

@@ -64,6 +64,8 @@ def test_attention_arguments():
     for bad in (dict(q=None), dict(out=None), dict(q=A + 4), dict(out=A + 8), dict(n_head=0), dict(n_head=6),
                 dict(n_head=-4), dict(window=-1), dict(sinks=-1)):
         assert _attention(_kv(), _rows(), **bad) == NH_E_ARG, bad
+    big = (1 << 31) - 1
+    assert _attention(_kv(), _rows(n_rows=big, max_rows=big), n_head=8) == NH_E_ARG  # more queries than 32 bits count
     assert _attention(_kv(), _rows(n_rows=0)) == 0  # nothing to do
 
 
@@ -73,6 +75,8 @@ def test_append_arguments():
                 dict(qs=513), dict(ks=258), dict(vs=257), dict(q=A + 4), dict(k=A + 4), dict(v=A + 8), dict(qr=A + 4),
                 dict(rope=A + 8), dict(qn=A + 4), dict(kn=A + 4)):
         assert _append(_kv(), _rows(), **bad) == NH_E_ARG, bad
+    for k in ("qs", "ks", "vs"):
+        assert _append(_kv(), _rows(), **{k: (1 << 23) + 4}) == NH_E_ARG
     assert _append(_kv(), _rows(n_rows=0)) == 0
     assert _append(_kv(), _rows(max_rows=0)) == 0
 

@@ -7,12 +7,15 @@
 //   operands (exact);
 //   warp 16 issues S = Qhi K + Qlo K and O += Phi V + Plo V (tcgen05.mma
 //   kind::f16; accumulators, Q and P in tensor memory);
-//   warps 0-3 and 4-7 hold a row a lane and half of the tile's positions each:
-//   scores, running maximum (exchanged) and sum, weights split into two f16
-//   parts that take the scores' place.
+//   warps 0-3 and 4-7 hold a row a lane and take the tiles in turn: scores,
+//   running maximum (handed from tile to tile) and sum, weights split into two
+//   f16 parts that take the scores' place.
 // Two or three score tiles rotate (what the tensor memory holds), so that the
 // tensor cores form the scores ahead while weights are in the making.
-// What bounds it: the two-part products make 8 hd products a score and row
+// What bounds it: at present a tile's way from its scores to its weights (some
+// 5,000 cycles at 2,500 a tile, head_dim 64), of which the exponentials and the
+// tensor memory's loads are the most, and before the first tile the query's way
+// in; below that the products: the two-part ones make 8 hd products a score and row
 // where one f16 pass would make 4 (the price of f32 queries and weights); beside
 // them some 8 operations a score for the softmax.  Operand tiles lie in shared
 // memory as rows of 64 dimensions, 128 bytes swizzled: the same image serves K
@@ -22,7 +25,9 @@
 // own accesses waited.)
 // The tensor cores' own additions cut off, which over a long sequence pulls every
 // sum towards zero (9e-6 of it at 4,096 positions): the sums of every few tiles
-// leave tensor memory and are added up in shared memory, rounded.
+// leave tensor memory and are added up in shared memory, rounded.  (Every third:
+// 1.1e-6 against the f32 formula's 1.4e-6 on 2,048 rows after 2,048 others;
+// every seventh would save 5% of the time at 2.1e-6.)
 // All waits are bounded; an expired one records NH_E_TIMEOUT.
 #include <cooperative_groups.h>
 
@@ -40,12 +45,13 @@ constexpr int kSub = 16;        // positions that certainly share a page
 constexpr int kSubs = kTileK / kSub;
 constexpr int kTileThreads = 640;
 constexpr int kSoftThreads = 256;
-constexpr int kHalf = kTileK / 2;  // positions of a tile that one softmax warp takes
 constexpr float kLeast = 1.17549435e-38f;  // factor of the scores at least: a hidden one, -inf, stays that
 constexpr int kHidden = -1000;     // V's exponent where no position is seen
 constexpr int kHalfBytes = kTileK * 128;  // 64 dimensions of an operand tile
 constexpr int kTileShift = 7;   // weights are 2^7 times [0, 2^8]
-constexpr int kFlush = 4;    // tiles whose products are added up in tensor memory
+constexpr int kFlush = 3;       // tiles whose products are added up in tensor memory
+constexpr int kScalePlaces = 8;
+constexpr int kLowest = -60;    // least power of two of a part's weights that products take
 constexpr float kGrow = 8.f;    // the maximum in use lags the true one by at most 2^8
 
 constexpr uint32_t kTmemCols = 512;
@@ -65,12 +71,14 @@ struct TileShared {
   uint8_t ring[2][2][kOperand];        // K, V: two stages each
   // Q on its way to tensor memory; the joined values once the products are done.
   float rows[kTileQ][kRow];
-  float ks[4][kSubs];  // scales of a tile's 16-position parts (four tiles)
-  int ve[4][kSubs];    // exponents of V's, or kHidden
-  float top[2][2][kTileQ];  // the halves' maxima of a row (two tiles)
+  float ks[kScalePlaces][kSubs];  // scales of a tile's 16-position parts
+  int ve[kScalePlaces][kSubs];    // exponents of V's, or kHidden
+  float2 ref[2][kTileQ];     // a row's maximum in use and V's exponent in use (as bits), after an even and an odd tile
+  float2 at_flush[kTileQ];   // the same, of the sums in `rows`
+  float top[2][kTileQ];      // largest magnitudes of the query's halves
   int64_t row_at[kTileQ];  // where a query's row starts in q and out
-  uint64_t full[2][2], empty[2][2], scales[4], q_full, s_full[kScoreTiles], p_full[kScoreTiles], pv_done[kScoreTiles], drained;
-  float m[kTileQ], l[2][kTileQ];
+  uint64_t full[2][2], empty[2][2], scales[kScalePlaces], q_rows, q_full, s_full[kScoreTiles], p_full[kScoreTiles], pv_done[kScoreTiles], drained;
+  float m[kTileQ], sum[kTileQ], l[2][kTileQ], lm[2][kTileQ];
   uint32_t tmem;
   int failed;
 };
@@ -221,12 +229,13 @@ __global__ void __launch_bounds__(kTileThreads, 1) paged_tile_kernel(const Paged
     for (int i = 0; i < 4; ++i) {
       mbar_init(&sh.full[i >> 1][i & 1], 4);
       mbar_init(&sh.empty[i >> 1][i & 1], 1);
-      mbar_init(&sh.scales[i], 4);
     }
+    for (int i = 0; i < kScalePlaces; ++i) mbar_init(&sh.scales[i], 4);
+    mbar_init(&sh.q_rows, 4);
     mbar_init(&sh.q_full, 8);
     for (int i = 0; i < kScoreTiles; ++i) {
       mbar_init(&sh.s_full[i], 1);
-      mbar_init(&sh.p_full[i], 8);
+      mbar_init(&sh.p_full[i], 4);
       mbar_init(&sh.pv_done[i], 1);
     }
     mbar_init(&sh.drained, 1);
@@ -349,16 +358,17 @@ __global__ void __launch_bounds__(kTileThreads, 1) paged_tile_kernel(const Paged
         *reinterpret_cast<uint4*>(d + ((piece + 1) ^ r) * 16) =
             make_uint4(codes_lo(raw[i].z), codes_hi(raw[i].z), codes_lo(raw[i].w), codes_hi(raw[i].w));
       }
-      // The scales' place was last read for tile j - 4, whose weights were in use before K of tile j found its stage free.
+      // The scales' place was last read for tile j - 8, whose weights were in use before K of tile j found its stage free
+      // (the scores of tile j - 2 follow the products of j - 5 at the latest).
       if (!of_v && lane < 2) {
-        sh.ks[j & 3][w * 2 + lane] = seen ? ks : 1.f;
-        sh.ve[j & 3][w * 2 + lane] = seen ? exponent_of(vs) : kHidden;
+        sh.ks[j & (kScalePlaces - 1)][w * 2 + lane] = seen ? ks : 1.f;
+        sh.ve[j & (kScalePlaces - 1)][w * 2 + lane] = seen ? exponent_of(vs) : kHidden;
       }
       fence_async_smem();
       __syncwarp();
       if (lane == 0) {
         mbar_arrive(&sh.full[of_v][j & 1]);
-        if (!of_v) mbar_arrive(&sh.scales[j & 3]);
+        if (!of_v) mbar_arrive(&sh.scales[j & (kScalePlaces - 1)]);
       }
       if (j + 1 < n) load(j + 1);
     }
@@ -395,11 +405,11 @@ __global__ void __launch_bounds__(kTileThreads, 1) paged_tile_kernel(const Paged
       };
       ok = all(mbar_wait(&sh.q_full, 0)) && scores(0) && (n < 2 || scores(1));
       for (int j = 0; j < n && ok; ++j) {
-        ok = mbar_wait(&sh.full[1][j & 1], static_cast<uint32_t>(j >> 1) & 1u) &&
-             mbar_wait(&sh.p_full[j % kScoreTiles], static_cast<uint32_t>(j / kScoreTiles) & 1u);
-        // With three score tiles, those of j + 2 will take the place of tile j - 1's weights.
-        if (kScoreTiles == 3 && ok && j > 0) ok = products_done(j - 1);
-        ok = all(ok);
+        // With three score tiles those of j + 2 take the place of tile j - 1's weights, before the products of j.
+        if (kScoreTiles == 3 && j + 2 < n) ok = (j == 0 || all(products_done(j - 1))) && scores(j + 2);
+        if (!ok) break;
+        ok = all(mbar_wait(&sh.full[1][j & 1], static_cast<uint32_t>(j >> 1) & 1u) &&
+                 mbar_wait(&sh.p_full[j % kScoreTiles], static_cast<uint32_t>(j / kScoreTiles) & 1u));
         if (!ok) break;
         tc_after();
         const uint64_t b = vd + ((j & 1) * kOp >> 4);
@@ -415,10 +425,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) paged_tile_kernel(const Paged
           tc_commit(&sh.pv_done[j % kScoreTiles]);
         }
         __syncwarp();
-        if (j + 2 < n) {
-          if (kScoreTiles == 2) ok = all(products_done(j));  // with two, that of this one's
-          ok = ok && scores(j + 2);
-        }
+        if (kScoreTiles == 2 && j + 2 < n) ok = all(products_done(j)) && scores(j + 2);  // with two, that of this one's
       }
       // No product is left in flight when the operands and the tensor memory are given up, whatever ended the loop.
       if (one) tc_commit(&sh.drained);
@@ -428,50 +435,40 @@ __global__ void __launch_bounds__(kTileThreads, 1) paged_tile_kernel(const Paged
     }
     __syncwarp();
   } else {
-    // ---------------------------------------------------------------- softmax: a row a lane, half of the positions
+    // ---------------------------------------------------------------- softmax: a row a lane, every second tile
     asm volatile("setmaxnreg.inc.sync.aligned.u32 144;\n");
     float row_m = -INFINITY, row_l = 0.f;  // the row's maximum in use, sum of its weights
     int eref = -200;                       // O is in units of 2^(eref - kTileShift + kCodeShift)
-    float pend = 1.f;  // what the sums in shared memory are still to be scaled by
     const int half = warp >> 2, quad = warp & 3, row = quad * 32 + lane;
     const uint32_t lanes = static_cast<uint32_t>(quad * 32) << 16;
     const int pos = row < nq ? sq.p0 + (q0 + row) / p.group : -1;
     const bool idle = quad * 32 >= nq;  // no row of this warp is a query
     float fq;
     {
-      // The rows, read whole; then the two lanes of a row scale half of it each so that the largest magnitude is in
+      // The rows, copied whole; then the two lanes of a row scale half of it each so that the largest magnitude is in
       // [2^13, 2^14), and split it.  A negative factor of the scores changes the query's sign.
-      int64_t at = 0;
-      if (lane < 16 && warp * 16 + lane < nq) {
-        const int qj = q0 + warp * 16 + lane, qr = qj / p.group;
-        at = (static_cast<int64_t>(sq.r0 + qr) * p.n_head + kh * p.group + qj - qr * p.group) * HD;
-        sh.row_at[warp * 16 + lane] = at;
-      }
-#pragma unroll 4
-      for (int i = 0; i < 16; ++i) {
-        const int64_t from = __shfl_sync(0xffffffffu, at, i);
-        float4* to = reinterpret_cast<float4*>(sh.rows[warp * 16 + i]) + lane;
-        if (lane < HD / 4) {
-          if (warp * 16 + i < nq)
-            cp_async16(to, reinterpret_cast<const float4*>(p.q + from) + lane);
-          else
-            *to = make_float4(0.f, 0.f, 0.f, 0.f);
+      if (half == 0) {
+        if (lane == 0) mbar_expect_tx(&sh.q_rows, static_cast<uint32_t>(max(0, min(nq - quad * 32, 32))) * HD * 4);
+        __syncwarp();
+        if (row < nq) {
+          const int qr = (q0 + row) / p.group, qh = q0 + row - qr * p.group;
+          const int64_t at = (static_cast<int64_t>(sq.r0 + qr) * p.n_head + kh * p.group + qh) * HD;
+          bulk_g2s(sh.rows[row], p.q + at, HD * 4, &sh.q_rows);
+          sh.row_at[row] = at;
         }
       }
-      cp_async_commit();
-      cp_async_wait<0>();
-      asm volatile("bar.sync 1, 256;\n" ::: "memory");
+      ok = mbar_wait(&sh.q_rows, 0);
+      __syncwarp();
       float4 x[HD / 8];
       float top = 0.f;
 #pragma unroll
       for (int i = 0; i < HD / 8; ++i) {
-        x[i] = reinterpret_cast<const float4*>(sh.rows[row])[half * (HD / 8) + i];
+        x[i] = row < nq ? reinterpret_cast<const float4*>(sh.rows[row])[half * (HD / 8) + i] : make_float4(0.f, 0.f, 0.f, 0.f);
         top = max3(top, max3(fabsf(x[i].x), fabsf(x[i].y), fabsf(x[i].z)), fabsf(x[i].w));
       }
-      sh.top[0][half][row] = top;
-      asm volatile("bar.sync %0, 64;\n" ::"r"(2 + quad) : "memory");
-      top = fmaxf(top, sh.top[0][half ^ 1][row]);
-      asm volatile("bar.sync %0, 64;\n" ::"r"(2 + quad) : "memory");  // read before the tiles' maxima take the place
+      sh.top[half][row] = top;
+      asm volatile("bar.sync %0, 64;\n" ::"r"(10 + quad) : "memory");
+      top = fmaxf(top, sh.top[half ^ 1][row]);
       const int e = min(max(exponent_of(top), -100), 127);
       const float up = p.scale < 0.f ? -pow2i(13 - e) : pow2i(13 - e);
 #pragma unroll
@@ -493,139 +490,172 @@ __global__ void __launch_bounds__(kTileThreads, 1) paged_tile_kernel(const Paged
       __syncwarp();
       if (lane == 0) mbar_arrive(&sh.q_full);
     }
-    // This lane's half of the row: sums in shared memory (when `more`) times f, plus those in tensor memory times g.
-    auto add_sums = [&](bool more, float f, float g) {
+    // Sums of the row in shared memory (when `more`) times f, plus those in tensor memory times g, 16 columns a step.
+    auto add_sums = [&](int i0, int i1, bool more, float f, float g) {
 #pragma unroll 1
-      for (int i = half * (HD / 32); i < (half + 1) * (HD / 32); ++i) {
-        uint32_t o[16];
-        tc_ld16(tmem + TileTmem<HD>::kO + lanes + i * 16, o);
-        tc_wait_ld();
-        tc_loaded16(o);
-        float4* to = reinterpret_cast<float4*>(&sh.rows[row][i * 16]);
+      for (int i = i0; i < i1; i += 2) {
+        uint32_t o[2][16];
+        float4 v[2][4];
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-          if (more) v = to[k];
-          to[k] = make_float4(fmaf(v.x, f, __uint_as_float(o[4 * k]) * g), fmaf(v.y, f, __uint_as_float(o[4 * k + 1]) * g),
-                              fmaf(v.z, f, __uint_as_float(o[4 * k + 2]) * g), fmaf(v.w, f, __uint_as_float(o[4 * k + 3]) * g));
+        for (int e = 0; e < 2; ++e) {
+          if (i + e >= i1) break;
+          tc_ld16(tmem + TileTmem<HD>::kO + lanes + (i + e) * 16, o[e]);
+        }
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          if (i + e >= i1) break;
+          const float4* from = reinterpret_cast<const float4*>(&sh.rows[row][(i + e) * 16]);
+#pragma unroll
+          for (int k = 0; k < 4; ++k) v[e][k] = more ? from[k] : make_float4(0.f, 0.f, 0.f, 0.f);
+        }
+        tc_wait_ld();
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          if (i + e >= i1) break;
+          tc_loaded16(o[e]);
+          float4* to = reinterpret_cast<float4*>(&sh.rows[row][(i + e) * 16]);
+#pragma unroll
+          for (int k = 0; k < 4; ++k)
+            to[k] = make_float4(fmaf(v[e][k].x, f, __uint_as_float(o[e][4 * k]) * g),
+                                fmaf(v[e][k].y, f, __uint_as_float(o[e][4 * k + 1]) * g),
+                                fmaf(v[e][k].z, f, __uint_as_float(o[e][4 * k + 2]) * g),
+                                fmaf(v[e][k].w, f, __uint_as_float(o[e][4 * k + 3]) * g));
         }
       }
     };
-    // No softmax warp leaves the loop early, so that the pairs' barriers stay matched: after an expired wait it runs on
-    // without waiting.
-    for (int j = 0; j < n; ++j) {
+    // From one maximum in use to another (-inf: nothing has been seen, and the sums are zero).
+    auto factor = [](float from, float to) { return from == to ? 1.f : exp2_fast(from - to); };
+    // The warps of a row take turns: one forms the maximum of its tile while the other forms the weights of the tile
+    // before.  Maximum and exponent in use go from tile to tile through shared memory, each row's sum of weights stays
+    // with the warp.  No warp leaves the loop early, so that the pairs' barriers stay matched: after an expired wait it
+    // runs on without waiting.
+    for (int j = half; j < n; j += 2) {
+      ok = ok && mbar_wait(&sh.s_full[j % kScoreTiles], static_cast<uint32_t>(j / kScoreTiles) & 1u);
+      __syncwarp();
       if (idle) {
-        // In step with the others: the phase before must be over.
-        if (ok && j > 0) ok = products_done(j - 1);
-        __syncwarp();
         if (lane == 0) mbar_arrive(&sh.p_full[j % kScoreTiles]);
         continue;
       }
-      ok = ok && mbar_wait(&sh.s_full[j % kScoreTiles], static_cast<uint32_t>(j / kScoreTiles) & 1u);
-      __syncwarp();
       tc_after();
-      const uint32_t scol = tmem + TileTmem<HD>::kS + (j % kScoreTiles) * kTileK + lanes + half * kHalf;
-      uint32_t u[kHalf];
-      tc_ld32(scol, u);
-      tc_ld32(scol + 32, u + 32);
-      ok = ok && mbar_wait(&sh.scales[j & 3], static_cast<uint32_t>(j >> 2) & 1u);
+      const uint32_t scol = tmem + TileTmem<HD>::kS + (j % kScoreTiles) * kTileK + lanes;
+      const int place = j & (kScalePlaces - 1);
+      ok = ok && mbar_wait(&sh.scales[place], static_cast<uint32_t>(j / kScalePlaces) & 1u);
       const int t0 = tile_pos(j);
-      // Scales: K's of this half's four parts, V's exponents of these and of the others.
-      const float4 k4 = *reinterpret_cast<const float4*>(&sh.ks[j & 3][half * 4]);
-      const int4 v4 = *reinterpret_cast<const int4*>(&sh.ve[j & 3][half * 4]);
-      const int4 w4 = *reinterpret_cast<const int4*>(&sh.ve[j & 3][(half ^ 1) * 4]);
-      const float ks[4] = {k4.x, k4.y, k4.z, k4.w};
-      const int ve[4] = {v4.x, v4.y, v4.z, v4.w};
-      const int low_e = min(min(min(v4.x, v4.y), min(v4.z, v4.w)), min(min(w4.x, w4.y), min(w4.z, w4.w)));
-      const int ev = max(max(max(v4.x, v4.y), max(v4.z, v4.w)), max(max(w4.x, w4.y), max(w4.z, w4.w)));
-      __syncwarp();
-      tc_wait_ld();
-      tc_loaded(u);
-      tc_loaded(u + 32);
-      float* x = reinterpret_cast<float*>(u);
+      // The tile's 16-position parts: V's exponents, what K's scale makes of a product.
+      int ve[kSubs];
+      float ka[kSubs];
+#pragma unroll
+      for (int i = 0; i < kSubs; i += 4) {
+        *reinterpret_cast<int4*>(ve + i) = *reinterpret_cast<const int4*>(&sh.ve[place][i]);
+        *reinterpret_cast<float4*>(ka + i) = *reinterpret_cast<const float4*>(&sh.ks[place][i]);
+      }
+      int ev = ve[0], low_e = ve[0];
+#pragma unroll
+      for (int i = 0; i < kSubs; ++i) {
+        ka[i] = fmaxf(fq * ka[i], kLeast);
+        ev = max(ev, ve[i]);
+        low_e = min(low_e, ve[i]);
+      }
       const bool plain = low_e != kHidden && t0 + kTileK - 1 <= first_pos &&
                          (p.window == 0 || t0 > last_pos - p.window || t0 + kTileK <= p.n_sink);
       if (!plain) {
-        const int h0 = t0 + half * kHalf;
-        // Bit i: position h0 + i is seen.
-        auto up_to = [](int i) { return i < 0 ? 0ull : i >= 63 ? ~0ull : (2ull << i) - 1ull; };
-        uint64_t see = up_to(pos - h0);
-        if (p.window > 0) see &= ~up_to(pos - p.window - h0) | up_to(p.n_sink - 1 - h0);
+        // Scores that the row does not see become -inf in tensor memory, 32 columns a step.
+#pragma unroll 1
+        for (int c = 0; c < kTileK / 32; ++c) {
+          const int h0 = t0 + c * 32;
+          auto up_to = [](int i) { return i < 0 ? 0u : i >= 31 ? ~0u : (2u << i) - 1u; };
+          uint32_t see = up_to(pos - h0);
+          if (p.window > 0) see &= ~up_to(pos - p.window - h0) | up_to(p.n_sink - 1 - h0);
+          if (sh.ve[place][2 * c] == kHidden) see &= 0xffff0000u;
+          if (sh.ve[place][2 * c + 1] == kHidden) see &= 0xffffu;
+          if (__all_sync(0xffffffffu, see == ~0u)) continue;
+          uint32_t x[32];
+          tc_ld32(scol + c * 32, x);
+          tc_wait_ld();
+          tc_loaded(x);
 #pragma unroll
-        for (int b = 0; b < 4; ++b)
-          if (ve[b] == kHidden) see &= ~(0xffffull << (b * kSub));
-        const uint32_t bits[2] = {static_cast<uint32_t>(see), static_cast<uint32_t>(see >> 32)};
-#pragma unroll
-        for (int i = 0; i < kHalf; ++i)
-          if ((bits[i >> 5] & (1u << (i & 31))) == 0u) x[i] = -INFINITY;
+          for (int i = 0; i < 32; ++i)
+            if ((see & (1u << i)) == 0u) x[i] = 0xff800000u;
+          tc_st32(scol + c * 32, x);
+        }
+        tc_wait_st();
       }
+      uint32_t u[2][32];
+      tc_ld32(scol, u[0]);
+      tc_ld32(scol + 32, u[1]);
       float top = -INFINITY;
+      auto maximum = [&](int c, const uint32_t* x) {
 #pragma unroll
-      for (int b = 0; b < 4; ++b) {
-        float t = fmaxf(x[b * kSub], x[b * kSub + 1]);
+        for (int d = 0; d < 2; ++d) {
+          float t = fmaxf(__uint_as_float(x[d * kSub]), __uint_as_float(x[d * kSub + 1]));
 #pragma unroll
-        for (int i = 2; i < kSub; i += 2) t = max3(t, x[b * kSub + i], x[b * kSub + i + 1]);
-        top = fmaxf(top, t * fmaxf(fq * ks[b], kLeast));
+          for (int i = 2; i < kSub; i += 2) t = max3(t, __uint_as_float(x[d * kSub + i]), __uint_as_float(x[d * kSub + i + 1]));
+          top = fmaxf(top, t * ka[2 * c + d]);
+        }
+      };
+      __syncwarp();
+      tc_wait_ld();
+      tc_loaded(u[0]);
+      tc_loaded(u[1]);
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        maximum(c, u[c]);
+        tc_ld32(scol + (c + 2) * 32, u[c]);
       }
-      sh.top[j & 1][half][row] = top;
-      asm volatile("bar.sync %0, 64;\n" ::"r"(2 + quad) : "memory");  // the other half's warp
-      top = fmaxf(top, sh.top[j & 1][half ^ 1][row]);
+      tc_wait_ld();
+      tc_loaded(u[0]);
+      tc_loaded(u[1]);
+#pragma unroll
+      for (int c = 0; c < 2; ++c) maximum(c + 2, u[c]);
+      float2 before = make_float2(-INFINITY, __int_as_float(-200));
+      if (j > 0) {
+        asm volatile("bar.sync %0, 64;\n" ::"r"(2 + half * 4 + quad) : "memory");  // the tile before's
+        before = sh.ref[half ^ 1][row];
+      }
+      row_l *= factor(row_m, before.x);
+      row_m = before.x;
+      eref = __float_as_int(before.y);
       // The maximum in use follows the true one only when that is 2^8 above it; O follows then, and when V's scale grows.
       const bool grow = top > (row_m == -INFINITY ? row_m : row_m + kGrow);
       const bool flush = j > 0 && j % kFlush == 0;
+      const bool move = __any_sync(0xffffffffu, grow) || ev > eref;
       float alpha = 1.f;
-      if (__any_sync(0xffffffffu, grow) || ev > eref) {
-        const int en = max(eref, ev);
-        if (grow) {
-          alpha = row_m == -INFINITY ? 0.f : exp2_fast(row_m - top);
-          row_m = top;
-          row_l *= alpha;
-        }
-        alpha *= pow2i(max(eref - en, -200));
-        eref = en;
-        if (j > 0 && !flush) {
-          pend *= alpha;
-          ok = ok && products_done(j - 1);
-          __syncwarp();
-          tc_after();
-#pragma unroll
-          for (int i = half * (HD / 32); i < (half + 1) * (HD / 32); ++i) {
-            uint32_t o[16];
-            tc_ld16(tmem + TileTmem<HD>::kO + lanes + i * 16, o);
-            tc_wait_ld();
-            tc_loaded16(o);
-#pragma unroll
-            for (int k = 0; k < 16; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * alpha);
-            tc_st16(tmem + TileTmem<HD>::kO + lanes + i * 16, o);
-          }
-        }
+      if (grow) {
+        alpha = factor(row_m, top);
+        row_m = top;
+        row_l *= alpha;
       }
+      const int en = max(eref, ev);
+      alpha *= pow2i(max(eref - en, -200));
+      eref = en;
+      sh.ref[half][row] = make_float2(row_m, __int_as_float(eref));
+      if (j + 1 < n) asm volatile("bar.arrive %0, 64;\n" ::"r"(2 + (half ^ 1) * 4 + quad) : "memory");
       const float base = row_m == -INFINITY ? 0.f : row_m;
+      const bool low = low_e - eref + kTileShift < kLowest;
       // Weights, in pairs as high and low f16 parts: of every 32 columns the first 16 hold the high ones.
-#pragma unroll
-      for (int c = 0; c < 2; ++c) {
+      auto weights = [&](int c, const uint32_t* x) {
         uint32_t w[32];
+        if (low) {
+          // Parts that are hidden, or whose scale is 2^60 below the largest: the weights count for the sum alone.
 #pragma unroll
-        for (int d = 0; d < 2; ++d) {
-          const int b = 2 * c + d, eb = ve[b] - eref + kTileShift;
-          const float a = fmaxf(fq * ks[b], kLeast);
-          float off = -base;
-          if (eb < -60) {
-            // Hidden, or a scale 2^60 below the largest: the weights count for the sum alone.
+          for (int d = 0; d < 2; ++d) {
+            if (ve[2 * c + d] - eref + kTileShift >= kLowest) continue;
             float sum = 0.f;
 #pragma unroll
-            for (int i = 0; i < kSub; ++i) sum += exp2_fast(fmaf(x[b * kSub + i], a, off));
+            for (int i = 0; i < kSub; ++i) sum += exp2_fast(fmaf(__uint_as_float(x[d * kSub + i]), ka[2 * c + d], -base));
             row_l += sum;
-            off = -INFINITY;
-          } else {
-            off += static_cast<float>(eb);
           }
+        }
+#pragma unroll
+        for (int d = 0; d < 2; ++d) {
+          const int eb = ve[2 * c + d] - eref + kTileShift;
+          const float a = ka[2 * c + d], off = eb < kLowest ? -INFINITY : static_cast<float>(eb) - base;
           float2 sum2 = make_float2(0.f, 0.f);
           const float2 a2 = make_float2(a, a), off2 = make_float2(off, off);
 #pragma unroll
           for (int i = 0; i < kSub / 2; ++i) {
-            const int k = b * kSub + 2 * i;
-            const float2 y = fma2(make_float2(x[k], x[k + 1]), a2, off2);
+            const int k = d * kSub + 2 * i;
+            const float2 y = fma2(make_float2(__uint_as_float(x[k]), __uint_as_float(x[k + 1])), a2, off2);
             const float2 e = make_float2(exp2_fast(y.x), exp2_fast(y.y));
             sum2 = add2(sum2, e);
             const __half2 h = __floats2half2_rn(e.x, e.y);
@@ -635,17 +665,43 @@ __global__ void __launch_bounds__(kTileThreads, 1) paged_tile_kernel(const Paged
             w[16 + d * 8 + i] = *reinterpret_cast<const uint32_t*>(&l);
           }
           const float sum = sum2.x + sum2.y;
-          row_l += sum * pow2i(min(-eb, 60));
+          row_l += sum * pow2i(min(-eb, -kLowest));
         }
         tc_st32(scol + c * 32, w);
+      };
+      // The last two quarters are at hand; the first two come back while these are worked on.
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        weights(c + 2, u[c]);
+        tc_ld32(scol + c * 32, u[c]);
       }
-      if (flush) {
-        // The tiles' sums so far, in this tile's units; its own products start from zero.
+      tc_wait_ld();
+      tc_loaded(u[0]);
+      tc_loaded(u[1]);
+#pragma unroll
+      for (int c = 0; c < 2; ++c) weights(c, u[c]);
+      if (flush || (move && j > 0)) {
         ok = ok && products_done(j - 1);
         __syncwarp();
         tc_after();
-        add_sums(j > kFlush, pend * alpha, alpha);
-        pend = 1.f;
+        if (flush) {
+          // The tiles' sums so far, in this tile's units; its own products start from zero.
+          const float2 at = sh.at_flush[row];
+          const float f = j > kFlush ? factor(at.x, row_m) * pow2i(max(__float_as_int(at.y) - eref, -200)) : 0.f;
+          add_sums(0, HD / 16, j > kFlush, f, alpha);
+          sh.at_flush[row] = make_float2(row_m, __int_as_float(eref));
+        } else {
+#pragma unroll 1
+          for (int i = 0; i < HD / 16; ++i) {
+            uint32_t o[16];
+            tc_ld16(tmem + TileTmem<HD>::kO + lanes + i * 16, o);
+            tc_wait_ld();
+            tc_loaded16(o);
+#pragma unroll
+            for (int k = 0; k < 16; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * alpha);
+            tc_st16(tmem + TileTmem<HD>::kO + lanes + i * 16, o);
+          }
+        }
       }
       tc_wait_st();
       tc_before();
@@ -658,11 +714,21 @@ __global__ void __launch_bounds__(kTileThreads, 1) paged_tile_kernel(const Paged
     __syncwarp();
     tc_after();
     sh.l[half][row] = row_l;
-    if (half == 0) sh.m[row] = row_m;
+    sh.lm[half][row] = row_m;
     asm volatile("bar.sync 1, 256;\n" ::: "memory");
-    const float unit = pow2i(max(eref, -126));
-    const float l = sh.l[0][row] + sh.l[1][row], inv = nrank > 1 ? 1.f : l == 0.f ? 0.f : 1.f / l;
-    if (n > 0 && !idle) add_sums(n > kFlush, pend, 1.f);
+    const float2 last = n > 0 && !idle ? sh.ref[(n - 1) & 1][row] : make_float2(-INFINITY, __int_as_float(-200));
+    const float unit = pow2i(max(__float_as_int(last.y), -126));
+    const float l = sh.l[0][row] * factor(sh.lm[0][row], last.x) + sh.l[1][row] * factor(sh.lm[1][row], last.x);
+    const float inv = nrank > 1 ? 1.f : l == 0.f ? 0.f : 1.f / l;
+    if (half == 0) {
+      sh.m[row] = last.x;
+      sh.sum[row] = l;
+    }
+    if (n > 0 && !idle) {
+      const float2 at = n > kFlush ? sh.at_flush[row] : last;
+      add_sums(half * (HD / 32), (half + 1) * (HD / 32), n > kFlush,
+               factor(at.x, last.x) * pow2i(max(__float_as_int(at.y) - __float_as_int(last.y), -200)), 1.f);
+    }
 #pragma unroll 4
     for (int i = half * (HD / 8); i < (half + 1) * (HD / 8); ++i) {
       float4& v = reinterpret_cast<float4*>(sh.rows[row])[i];
@@ -695,7 +761,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) paged_tile_kernel(const Paged
           const TileShared<HD>* o = cluster.map_shared_rank(&sh, r);
           const float a = o->m[row] == -INFINITY ? 0.f : exp2_fast(o->m[row] - top);
           const float4 y = reinterpret_cast<const float4*>(o->rows[row])[d];
-          sum += a * (o->l[0][row] + o->l[1][row]);
+          sum += a * o->sum[row];
           v.x += a * y.x;
           v.y += a * y.y;
           v.z += a * y.z;

@@ -1,8 +1,14 @@
 // Attention over the paged 8-bit K/V cache for few rows a sequence: decode
 // positions and drafted ones (nh_paged_attention's split form).
 //
-// What bounds it: every cached byte is read once, so the copy rate of HBM.  A
-// CTA takes up to 2, 4, 8 or 16 queries of one (sequence, KV head) and a contiguous
+// What bounds it: every cached byte is read once, so the copy rate of HBM; with
+// more queries the instructions of the codes' conversion and of the products'
+// operands.  Measured (16 KV heads of 128, one query each): 64 sequences of up
+// to 4,096 positions 128 us (5.4 TB/s of a copy's 6.5; the reads alone take 114,
+// unequal lengths on 296 places for CTAs), one of 131,001 positions 135 us
+// (4.0 TB/s: 256 CTAs on 148 SMs); 16 of up to 6,001, 8 heads of 128, 20 queries
+// each 78 us.  Measured and left: CTAs in order of length (129 us), two stages
+// and three CTAs to an SM (156), page ids fetched in the units' loop.  A CTA takes up to 2, 4, 8 or 16 queries of one (sequence, KV head) and a contiguous
 // part of the positions; a cluster's CTAs split the positions and join their
 // (maximum, sum, weighted values) through distributed shared memory in rank
 // order.  A warp takes units of 16 positions, always inside one page, through a
@@ -33,9 +39,12 @@ namespace nh {
 namespace {
 
 constexpr int kUnit = 16;  // positions of one warp step
+// Sequences with at most this many queries a KV head take this form, others the tiled one, whose time hardly depends on
+// the queries: 16 sequences of up to 6,001 positions, 8 KV heads of 128, take 114 us here and 129 tiled with 32 queries,
+// 147 and 131 with 48; one of 8,000 positions and 16 KV heads 35 and 54 with 32, 63 and 55 with 48.
+constexpr int kFewQueries = 32;
 // Warps of a CTA: sixteen to an SM either way by their registers, in fewer and larger CTAs for four queries (one long
 // sequence 158 -> 135 us, the decode batch 134 -> 127 us against four warps a CTA).
-constexpr int kFewQueries = 32;
 template <int NQ>
 constexpr int kWarpsOf = NQ <= 4 ? 8 : 4;
 

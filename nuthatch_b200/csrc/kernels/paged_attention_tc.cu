@@ -12,14 +12,20 @@
 //   f16 parts that take the scores' place.
 // Two or three score tiles rotate (what the tensor memory holds), so that the
 // tensor cores form the scores ahead while weights are in the making.
-// What bounds it: at present a tile's way from its scores to its weights (some
-// 5,000 cycles at 2,500 a tile, head_dim 64), of which the exponentials and the
-// tensor memory's loads are the most, and before the first tile the query's way
-// in; below that the products: the two-part ones make 8 hd products a score and row
-// where one f16 pass would make 4 (the price of f32 queries and weights); beside
-// them some 8 operations a score for the softmax.  Operand tiles lie in shared
-// memory as rows of 64 dimensions, 128 bytes swizzled: the same image serves K
-// (K-major) and V (MN-major), and eight lanes write to different banks.
+// What bounds it.  The products: f32 queries and weights as two f16 parts each
+// make 8 hd operations a score where one f16 pass would make 4, 2,048 cycles a
+// tile of 128 dimensions; the exponentials, 1,024 cycles a tile.  At present the
+// way of a tile from its scores to its weights is longer than either: some 5,000
+// cycles (tensor memory's loads, the exponentials, the hand-over), of which the
+// two groups of warps hide half, and 10,000 before a CTA's first tile.  2,048
+// rows after 2,048 others, 16 heads of 128: 125 us (half of the tensor cores'
+// measured rate with both parts counted); four prompts of up to 4,000 rows, 16
+// heads of 64 over 8, window 1,024: 245 us.  (Both groups on one tile, half of
+// its columns each: 137 and 274 us.  Walking a tile in loops instead of unrolled:
+// 129 and 251.)
+// Operand tiles lie in shared memory as rows of 64 dimensions, 128 bytes swizzled:
+// the same image serves K (K-major) and V (MN-major), and eight lanes write to
+// different banks.
 // (Unswizzled operands are read at half the rate: with Q in shared memory too, a
 // 16-wide step of the scores took 138 cycles for 64, and the softmax warps'
 // own accesses waited.)

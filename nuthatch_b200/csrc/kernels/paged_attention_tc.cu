@@ -18,11 +18,15 @@
 // way of a tile from its scores to its weights is longer than either: some 5,000
 // cycles (tensor memory's loads, the exponentials, the hand-over), of which the
 // two groups of warps hide half, and 10,000 before a CTA's first tile.  2,048
-// rows after 2,048 others, 16 heads of 128: 125 us (half of the tensor cores'
+// rows after 2,048 others, 16 heads of 128: 124 us (half of the tensor cores'
 // measured rate with both parts counted); four prompts of up to 4,000 rows, 16
-// heads of 64 over 8, window 1,024: 245 us.  (Both groups on one tile, half of
+// heads of 64 over 8, window 1,024: 240 us.  (Both groups on one tile, half of
 // its columns each: 137 and 274 us.  Walking a tile in loops instead of unrolled:
-// 129 and 251.)
+// 129 and 251.  Narrow heads as two CTAs to an SM, each with one group of softmax
+// warps and one score tile, which would hide the starts: 253 us for 247, 91 for 76
+// with one prompt, as each tile then waits for its own products.  A CTA's start
+// is mostly its queries': 16 copies by each of eight warps 240 us, 32 by four
+// 245, 128 by one 281, 16-byte copies 253, loads into registers 248.)
 // Operand tiles lie in shared memory as rows of 64 dimensions, 128 bytes swizzled:
 // the same image serves K (K-major) and V (MN-major), and eight lanes write to
 // different banks.
@@ -237,7 +241,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) paged_tile_kernel(const Paged
       mbar_init(&sh.empty[i >> 1][i & 1], 1);
     }
     for (int i = 0; i < kScalePlaces; ++i) mbar_init(&sh.scales[i], 4);
-    mbar_init(&sh.q_rows, 4);
+    mbar_init(&sh.q_rows, 8);
     mbar_init(&sh.q_full, 8);
     for (int i = 0; i < kScoreTiles; ++i) {
       mbar_init(&sh.s_full[i], 1);
@@ -451,16 +455,18 @@ __global__ void __launch_bounds__(kTileThreads, 1) paged_tile_kernel(const Paged
     const bool idle = quad * 32 >= nq;  // no row of this warp is a query
     float fq;
     {
-      // The rows, copied whole; then the two lanes of a row scale half of it each so that the largest magnitude is in
-      // [2^13, 2^14), and split it.  A negative factor of the scores changes the query's sign.
-      if (half == 0) {
-        if (lane == 0) mbar_expect_tx(&sh.q_rows, static_cast<uint32_t>(max(0, min(nq - quad * 32, 32))) * HD * 4);
+      // The rows, copied whole, sixteen by a warp (the copies are sent one after the other); then the two lanes of a row
+      // scale half of it each so that the largest magnitude is in [2^13, 2^14), and split it.  A negative factor of the
+      // scores changes the query's sign.
+      {
+        const int mine = warp * 16 + lane;
+        if (lane == 0) mbar_expect_tx(&sh.q_rows, static_cast<uint32_t>(max(0, min(nq - warp * 16, 16))) * HD * 4);
         __syncwarp();
-        if (row < nq) {
-          const int qr = (q0 + row) / p.group, qh = q0 + row - qr * p.group;
+        if (lane < 16 && mine < nq) {
+          const int qr = (q0 + mine) / p.group, qh = q0 + mine - qr * p.group;
           const int64_t at = (static_cast<int64_t>(sq.r0 + qr) * p.n_head + kh * p.group + qh) * HD;
-          bulk_g2s(sh.rows[row], p.q + at, HD * 4, &sh.q_rows);
-          sh.row_at[row] = at;
+          bulk_g2s(sh.rows[mine], p.q + at, HD * 4, &sh.q_rows);
+          sh.row_at[mine] = at;
         }
       }
       ok = mbar_wait(&sh.q_rows, 0);
@@ -496,8 +502,9 @@ __global__ void __launch_bounds__(kTileThreads, 1) paged_tile_kernel(const Paged
       __syncwarp();
       if (lane == 0) mbar_arrive(&sh.q_full);
     }
-    // Sums of the row in shared memory (when `more`) times f, plus those in tensor memory times g, 16 columns a step.
-    auto add_sums = [&](int i0, int i1, bool more, float f, float g) {
+    // Sums of the row in shared memory (when `more`) times f, plus those in tensor memory times g, 16 columns a step;
+    // `done` is applied to the results.
+    auto add_sums = [&](int i0, int i1, bool more, float f, float g, auto done) {
 #pragma unroll 1
       for (int i = i0; i < i1; i += 2) {
         uint32_t o[2][16];
@@ -522,10 +529,10 @@ __global__ void __launch_bounds__(kTileThreads, 1) paged_tile_kernel(const Paged
           float4* to = reinterpret_cast<float4*>(&sh.rows[row][(i + e) * 16]);
 #pragma unroll
           for (int k = 0; k < 4; ++k)
-            to[k] = make_float4(fmaf(v[e][k].x, f, __uint_as_float(o[e][4 * k]) * g),
-                                fmaf(v[e][k].y, f, __uint_as_float(o[e][4 * k + 1]) * g),
-                                fmaf(v[e][k].z, f, __uint_as_float(o[e][4 * k + 2]) * g),
-                                fmaf(v[e][k].w, f, __uint_as_float(o[e][4 * k + 3]) * g));
+            to[k] = make_float4(done(fmaf(v[e][k].x, f, __uint_as_float(o[e][4 * k]) * g)),
+                                done(fmaf(v[e][k].y, f, __uint_as_float(o[e][4 * k + 1]) * g)),
+                                done(fmaf(v[e][k].z, f, __uint_as_float(o[e][4 * k + 2]) * g)),
+                                done(fmaf(v[e][k].w, f, __uint_as_float(o[e][4 * k + 3]) * g)));
         }
       }
     };
@@ -694,7 +701,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) paged_tile_kernel(const Paged
           // The tiles' sums so far, in this tile's units; its own products start from zero.
           const float2 at = sh.at_flush[row];
           const float f = j > kFlush ? factor(at.x, row_m) * pow2i(max(__float_as_int(at.y) - eref, -200)) : 0.f;
-          add_sums(0, HD / 16, j > kFlush, f, alpha);
+          add_sums(0, HD / 16, j > kFlush, f, alpha, [](float x) { return x; });
           sh.at_flush[row] = make_float2(row_m, __int_as_float(eref));
         } else {
 #pragma unroll 1
@@ -730,17 +737,14 @@ __global__ void __launch_bounds__(kTileThreads, 1) paged_tile_kernel(const Paged
       sh.m[row] = last.x;
       sh.sum[row] = l;
     }
-    if (n > 0 && !idle) {
+    if (n == 0) {
+      for (int i = half * (HD / 8); i < (half + 1) * (HD / 8); ++i)
+        reinterpret_cast<float4*>(sh.rows[row])[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+    } else if (!idle) {
       const float2 at = n > kFlush ? sh.at_flush[row] : last;
       add_sums(half * (HD / 32), (half + 1) * (HD / 32), n > kFlush,
-               factor(at.x, last.x) * pow2i(max(__float_as_int(at.y) - __float_as_int(last.y), -200)), 1.f);
-    }
-#pragma unroll 4
-    for (int i = half * (HD / 8); i < (half + 1) * (HD / 8); ++i) {
-      float4& v = reinterpret_cast<float4*>(sh.rows[row])[i];
-      const float4 y = n > 0 ? v : make_float4(0.f, 0.f, 0.f, 0.f);
-      const float f = pow2i(kCodeShift - kTileShift);
-      v = make_float4(y.x * f * unit * inv, y.y * f * unit * inv, y.z * f * unit * inv, y.w * f * unit * inv);
+               factor(at.x, last.x) * pow2i(max(__float_as_int(at.y) - __float_as_int(last.y), -200)), 1.f,
+               [=](float x) { return x * (pow2i(kCodeShift - kTileShift) * unit) * inv; });
     }
     tc_before();
   }

@@ -352,6 +352,24 @@ def test_attention_far_pages(gpu):
     assert int(dev.err.item()) == 0
 
 
+@pytest.mark.parametrize("hd", [64, 128])
+def test_attention_equal_calls_give_equal_bits(gpu, hd):
+    """The warps and CTAs that share a row join what they have in an order that does not depend on which comes first."""
+    import torch
+
+    for n, p0 in (([1] * 3, [2000, 40, 777]), ([6, 3], [900, 31]), ([300, 7, 129], [500, 1200, 0]), ([64], [3000])):
+        rng, table, cache, dev = _setup(n, p0, 16, 4, hd, 16, 31)
+        q = _cuda(rng.standard_normal((sum(n), 16 * hd)).astype(np.float32) * 4)
+        rows, keep = dev.rows(n, p0)
+        outs = []
+        for _ in range(12):
+            out = torch.empty_like(q)
+            assert lib().nh_paged_attention(C.byref(dev.kv), C.byref(rows), P(q), 16, 0.1, 600, 3, P(out), _stream()) == 0
+            outs.append(out)
+        torch.cuda.synchronize()
+        assert all(torch.equal(outs[0], o) for o in outs[1:]), n
+
+
 def test_two_streams_at_once(gpu):
     """Calls on two streams over caches of their own, with nothing shared, give what they give alone."""
     import torch

@@ -7,7 +7,7 @@
 // to 4,096 positions 128 us (5.4 TB/s of a copy's 6.5; the reads alone take 114,
 // unequal lengths on 296 places for CTAs), one of 131,001 positions 135 us
 // (4.0 TB/s: 256 CTAs on 148 SMs); 16 of up to 6,001, 8 heads of 128, 20 queries
-// each 78 us.  Measured and left: CTAs in order of length (129 us), two stages
+// each 78 us, 32 queries 93.  Measured and left: CTAs in order of length (129 us), two stages
 // and three CTAs to an SM (156), page ids fetched in the units' loop.  A CTA takes up to 2, 4, 8 or 16 queries of one (sequence, KV head) and a contiguous
 // part of the positions; a cluster's CTAs split the positions and join their
 // (maximum, sum, weighted values) through distributed shared memory in rank
@@ -40,8 +40,8 @@ namespace {
 
 constexpr int kUnit = 16;  // positions of one warp step
 // Sequences with at most this many queries a KV head take this form, others the tiled one, whose time hardly depends on
-// the queries: 16 sequences of up to 6,001 positions, 8 KV heads of 128, take 114 us here and 129 tiled with 32 queries,
-// 147 and 131 with 48; one of 8,000 positions and 16 KV heads 35 and 54 with 32, 63 and 55 with 48.
+// the queries: 16 sequences of up to 6,001 positions, 8 KV heads of 128, take 93 us here and 129 tiled with 32 queries,
+// 130 and 130 with 48, 171 and 129 with 64; one of 8,000 positions and 16 KV heads 35 and 53 with 32.
 constexpr int kFewQueries = 32;
 // Warps of a CTA: sixteen to an SM either way by their registers, in fewer and larger CTAs for four queries (one long
 // sequence 158 -> 135 us, the decode batch 134 -> 127 us against four warps a CTA).
@@ -588,7 +588,7 @@ __device__ __forceinline__ void split_queries(const PagedAttnArgs& p) {
 }
 
 template <int HD, int NQ>
-__global__ void __launch_bounds__(kWarpsOf<NQ> * 32, NQ == 8 ? 3 : 2) paged_split_kernel(const PagedAttnArgs p) {
+__global__ void __launch_bounds__(kWarpsOf<NQ> * 32, NQ >= 8 ? 3 : 2) paged_split_kernel(const PagedAttnArgs p) {
   if constexpr (NQ == 16) {
     // The rest of a sequence's queries, or a sequence with few in a batch of others: half the products (20 queries of 16
     // sequences 83 -> 78 us).
@@ -604,25 +604,33 @@ template <int HD, int NQ>
 int launch_split(const PagedAttnArgs& p, int groups, int ranks, cudaStream_t s) {
   static SmemLimit configured;
   static WideCluster wide;
-  const size_t smem = sizeof(SplitShared<HD, NQ>);
+  size_t smem = sizeof(SplitShared<HD, NQ>);
+  // Few CTAs are spread out: two to an SM where that holds them all (32 queries over 8,000 positions, 16 heads: 35 us,
+  // with three to an SM 41).
+  if (NQ == 16 && static_cast<int64_t>(ranks) * p.kv.n_kv * groups * p.rows.n_seq <= 2 * device_sm_count())
+    smem = std::max<size_t>(smem, 76 * 1024);
   if (!ensure_smem(paged_split_kernel<HD, NQ>, smem, configured)) return NH_E_CUDA;
   if (ranks > 8 && !ensure_wide_cluster(paged_split_kernel<HD, NQ>, wide)) return NH_E_CUDA;
   return launch_cluster(paged_split_kernel<HD, NQ>, dim3(ranks, p.kv.n_kv * groups, p.rows.n_seq),
                         dim3(kWarpsOf<NQ> * 32), ranks, smem, s, p);
 }
 
-// CTAs of a (sequence, KV head, query group): one, unless the groups alone leave less than eight warps to an SM.  More
+// CTAs of a (sequence, KV head, query group): one, unless the groups alone leave less than eight warps to an SM, or, with
+// the 16-query form, twelve (three CTAs of 168 registers; a last group of eight queries or fewer counts half, as it has
+// half of the work, or none where the sequence is shorter).  16 sequences and 8 KV heads, 32 queries each: 93 us with 2
+// CTAs a group, 105 with 4, 114 with 4 and two CTAs to an SM; 20 queries: 88 with 2, 78 with 4.  More
 // are not free (each forms the query's operand and joins what it has), so a warp keeps a unit, and a cluster
 // larger than the portable eight, which is slow to start, has more: one sequence's 8,000 positions of 16 heads take
 // 17.6 us with 8 CTAs a head and 22.6 with 16, 131,001 positions 150 and 133.
 template <int HD, int NQ>
-int launch_group(const PagedAttnArgs& p, int groups, cudaStream_t s) {
+int launch_group(const PagedAttnArgs& p, int most, cudaStream_t s) {
+  const int groups = (most + NQ - 1) / NQ, halves = 2 * groups - (NQ == 16 && most - (groups - 1) * NQ <= 8 ? 1 : 0);
   if (static_cast<int64_t>(p.kv.n_kv) * groups > 65535) return NH_E_ARG;
-  constexpr int kWarps = kWarpsOf<NQ>;
-  const int64_t items = static_cast<int64_t>(p.rows.n_seq) * p.kv.n_kv * groups;
+  constexpr int kWarps = kWarpsOf<NQ>, kFill = NQ == 16 ? 12 : 8;
+  const int64_t items = static_cast<int64_t>(p.rows.n_seq) * p.kv.n_kv * halves;  // in halves
   const int64_t units = static_cast<int64_t>(p.rows.max_blocks) * p.kv.page / kUnit;
   int ranks = 1;
-  while (ranks < 16 && items * ranks * kWarps < 8 * device_sm_count() &&
+  while (ranks < 16 && items * ranks * kWarps < 2 * kFill * device_sm_count() &&
          units >= (ranks < 8 ? 1 : 16) * kWarps * 2 * ranks)
     ranks *= 2;
   return launch_split<HD, NQ>(p, groups, ranks, s);
@@ -631,10 +639,10 @@ int launch_group(const PagedAttnArgs& p, int groups, cudaStream_t s) {
 template <int HD>
 int launch_split_hd(const PagedAttnArgs& p, cudaStream_t s) {
   const int most = static_cast<int>(std::min<int64_t>(p.few, static_cast<int64_t>(p.rows.max_rows) * p.group));
-  return most <= 2   ? launch_group<HD, 2>(p, 1, s)
-         : most <= 4 ? launch_group<HD, 4>(p, 1, s)
-         : most <= 8 ? launch_group<HD, 8>(p, 1, s)
-                     : launch_group<HD, 16>(p, (most + 15) / 16, s);
+  return most <= 2   ? launch_group<HD, 2>(p, most, s)
+         : most <= 4 ? launch_group<HD, 4>(p, most, s)
+         : most <= 8 ? launch_group<HD, 8>(p, most, s)
+                     : launch_group<HD, 16>(p, most, s);
 }
 
 }  // namespace

@@ -482,7 +482,8 @@ typedef struct NhPagedRows {
  * counts as out of bounds).  q and qr may both be null.  A K or V value that
  * is not finite is coded as the nearest end of the range (a NaN as its middle),
  * sets no scale, and records NH_E_ARG in *err.  Pointers are 16-byte aligned, strides
- * a multiple of 4 and at most 2^23. */
+ * a multiple of 4 and at most 2^23; a call writes at most 65,535 pages of a
+ * sequence. */
 int nh_paged_append(const NhPagedKv* kv, const NhPagedRows* rows, const float* q, int64_t q_stride, const float* k,
                     int64_t k_stride, const float* v, int64_t v_stride, const float* q_norm, const float* k_norm,
                     float eps, int n_head, const float* rope_cs, int rope_len, float* qr, void* stream);
@@ -494,7 +495,8 @@ int nh_paged_append(const NhPagedKv* kv, const NhPagedRows* rows, const float* q
  * which stay visible).  qr and out are [n_rows][n_head*head_dim], 16-byte
  * aligned; any n_head that n_head_kv divides.  No scratch: a sequence with few
  * rows is split over the CTAs of a cluster, joined in a fixed order, so equal
- * calls give equal bits.  A row that sees no position gives zeros. */
+ * calls give equal bits.  A row that sees no position gives zeros.  max_rows *
+ * n_head / n_head_kv is below 2^31. */
 int nh_paged_attention(const NhPagedKv* kv, const NhPagedRows* rows, const float* qr, int n_head, float kq_scale,
                        int window, int n_sink, float* out, void* stream);
 

@@ -348,12 +348,13 @@ __device__ __forceinline__ void split_queries(const PagedAttnArgs& p) {
 #pragma unroll
   for (int i = 0; i < ON; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
   float m[QT], l[QT];  // running maximum; sum of the weights
+  int eref[QT];  // a query's sums are in units of 2^(eref - kWeightShift + kCodeShift), of the scales that it sees
 #pragma unroll
   for (int k = 0; k < QT; ++k) {
     m[k] = -INFINITY;
     l[k] = 0.f;
+    eref[k] = -200;
   }
-  int eref = -200;  // the sums are in units of 2^(eref - kWeightShift + kCodeShift)
 
   int st = 0;
   for (int i = i0; i < u1; i += kSplitWarps) {
@@ -407,6 +408,7 @@ __device__ __forceinline__ void split_queries(const PagedAttnArgs& p) {
     const bool plain = seen_here && t0 + kUnit - 1 <= first_pos &&
                        (p.window == 0 || t0 > last_pos - p.window || t0 + kUnit <= p.n_sink);  // all of them see all
     float x[QT][ST], top[QT];
+    int ev[QT];  // the exponent of V's scale where the query sees any of the unit
     bool grew = false;
 #pragma unroll
     for (int k = 0; k < QT; ++k) {
@@ -433,15 +435,18 @@ __device__ __forceinline__ void split_queries(const PagedAttnArgs& p) {
 #pragma unroll
       for (int e = kSmall ? 4 : 1; e <= (kSmall ? 16 : 2); e <<= 1)
         top[k] = fmaxf(top[k], __shfl_xor_sync(0xffffffffu, top[k], e));
-      grew |= top[k] > m[k];
+      const bool sees = plain || (seen_here && t0 <= pos[k] &&
+                                  (p.window == 0 || t0 + kUnit - 1 > pos[k] - p.window || t0 < p.n_sink));
+      ev[k] = sees ? exponent_of(v_scale) : eref[k];
+      grew |= top[k] > m[k] || ev[k] > eref[k];
     }
-    const int ev = seen_here ? exponent_of(v_scale) : eref;
     // Rarely after the first units: a larger score, or a larger scale of V.
-    if (__any_sync(0xffffffffu, grew) || ev > eref) {
-      const int en = max(eref, ev);
-      const float fe = pow2i(max(eref - en, -200));
+    if (__any_sync(0xffffffffu, grew)) {
 #pragma unroll
       for (int k = 0; k < QT; ++k) {
+        const int en = max(eref[k], ev[k]);
+        const float fe = pow2i(max(eref[k] - en, -200));
+        eref[k] = en;
         const float a = m[k] == -INFINITY ? 0.f : exp2_fast(m[k] - top[k]);
         m[k] = top[k];
         l[k] *= a;
@@ -458,13 +463,11 @@ __device__ __forceinline__ void split_queries(const PagedAttnArgs& p) {
           }
         }
       }
-      eref = en;
     }
-    const float fw = pow2i(ev - eref + kWeightShift);
     uint32_t hi[QT][2], lo[QT][2];
 #pragma unroll
     for (int k = 0; k < QT; ++k) {
-      const float base = m[k] == -INFINITY ? 0.f : m[k];
+      const float base = m[k] == -INFINITY ? 0.f : m[k], fw = pow2i(ev[k] - eref[k] + kWeightShift);
       float w[4];
 #pragma unroll
       for (int e = 0; e < ST; ++e) {
@@ -525,9 +528,9 @@ __device__ __forceinline__ void split_queries(const PagedAttnArgs& p) {
   // This warp's values in their own units, then the CTA's and the cluster's.
   cp_async_wait<0>();
   __syncthreads();
-  const float unit = pow2i(max(eref, -126));
 #pragma unroll
   for (int k = 0; k < QT; ++k) {
+    const float unit = pow2i(max(eref[k], -126));
 #pragma unroll
     for (int e = kSmall ? 4 : 1; e <= (kSmall ? 16 : 2); e <<= 1) {
       l[k] += __shfl_xor_sync(0xffffffffu, l[k], e);

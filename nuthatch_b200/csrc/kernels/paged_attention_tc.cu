@@ -83,7 +83,8 @@ struct TileShared {
   float rows[kTileQ][kRow];
   float ks[kScalePlaces][kSubs];  // scales of a tile's 16-position parts
   int ve[kScalePlaces][kSubs];    // exponents of V's, or kHidden
-  float2 ref[2][kTileQ];     // a row's maximum in use and V's exponent in use (as bits), after an even and an odd tile
+  // A row's maximum in use and V's exponent in use (as bits; of the parts that the row sees), after an even and an odd tile.
+  float2 ref[2][kTileQ];
   float2 at_flush[kTileQ];   // the same, of the sums in `rows`
   float top[2][kTileQ];      // largest magnitudes of the query's halves
   int64_t row_at[kTileQ];  // where a query's row starts in q and out
@@ -562,14 +563,13 @@ __global__ void __launch_bounds__(kTileThreads, 1) paged_tile_kernel(const Paged
         *reinterpret_cast<int4*>(ve + i) = *reinterpret_cast<const int4*>(&sh.ve[place][i]);
         *reinterpret_cast<float4*>(ka + i) = *reinterpret_cast<const float4*>(&sh.ks[place][i]);
       }
-      int ev = ve[0], low_e = ve[0];
+      bool whole = true;
 #pragma unroll
       for (int i = 0; i < kSubs; ++i) {
         ka[i] = fmaxf(fq * ka[i], kLeast);
-        ev = max(ev, ve[i]);
-        low_e = min(low_e, ve[i]);
+        whole &= ve[i] != kHidden;
       }
-      const bool plain = low_e != kHidden && t0 + kTileK - 1 <= first_pos &&
+      const bool plain = whole && t0 + kTileK - 1 <= first_pos &&
                          (p.window == 0 || t0 > last_pos - p.window || t0 + kTileK <= p.n_sink);
       if (!plain) {
         // Scores that the row does not see become -inf in tensor memory, 32 columns a step.
@@ -592,6 +592,18 @@ __global__ void __launch_bounds__(kTileThreads, 1) paged_tile_kernel(const Paged
           tc_st32(scol + c * 32, x);
         }
         tc_wait_st();
+        // Parts of which the row sees nothing: their scales must not count for it.
+#pragma unroll
+        for (int i = 0; i < kSubs; ++i) {
+          const int a = t0 + i * kSub;
+          if (a > pos || (p.window > 0 && a + kSub - 1 <= pos - p.window && a >= p.n_sink)) ve[i] = kHidden;
+        }
+      }
+      int ev = kHidden, low_e = 1000;  // the row's largest exponent of V in the tile, and the least
+#pragma unroll
+      for (int i = 0; i < kSubs; ++i) {
+        ev = max(ev, ve[i]);
+        if (ve[i] != kHidden) low_e = min(low_e, ve[i]);
       }
       uint32_t u[2][32];
       tc_ld32(scol, u[0]);
@@ -631,7 +643,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) paged_tile_kernel(const Paged
       // The maximum in use follows the true one only when that is 2^8 above it; O follows then, and when V's scale grows.
       const bool grow = top > (row_m == -INFINITY ? row_m : row_m + kGrow);
       const bool flush = j > 0 && j % kFlush == 0;
-      const bool move = __any_sync(0xffffffffu, grow) || ev > eref;
+      const bool move = __any_sync(0xffffffffu, grow || ev > eref);
       float alpha = 1.f;
       if (grow) {
         alpha = factor(row_m, top);
@@ -649,10 +661,10 @@ __global__ void __launch_bounds__(kTileThreads, 1) paged_tile_kernel(const Paged
       auto weights = [&](int c, const uint32_t* x) {
         uint32_t w[32];
         if (low) {
-          // Parts that are hidden, or whose scale is 2^60 below the largest: the weights count for the sum alone.
+          // Parts whose scale is 2^60 below the largest: the weights count for the sum alone.
 #pragma unroll
           for (int d = 0; d < 2; ++d) {
-            if (ve[2 * c + d] - eref + kTileShift >= kLowest) continue;
+            if (ve[2 * c + d] == kHidden || ve[2 * c + d] - eref + kTileShift >= kLowest) continue;
             float sum = 0.f;
 #pragma unroll
             for (int i = 0; i < kSub; ++i) sum += exp2_fast(fmaf(__uint_as_float(x[d * kSub + i]), ka[2 * c + d], -base));

@@ -1,0 +1,70 @@
+"""The paged 8-bit K/V cache and the draft check where a call's data decide: what
+hidden positions hold, values at the ends of f32, entries that are not finite."""
+from __future__ import annotations
+
+import ctypes as C
+
+import numpy as np
+import pytest
+
+from nuthatch_b200._lib import lib
+from tests import paged_model as pm
+from tests.test_gpu_paged import P, _cuda, _setup, _stream
+
+pytestmark = pytest.mark.gpu
+
+
+def _attend(dev, q, n, p0, n_head, scale, window, sinks, rows=None):
+    import torch
+
+    rows, keep = dev.rows(n, p0) if rows is None else rows
+    qd = _cuda(q.reshape(q.shape[0], -1))
+    out = torch.full_like(qd, 7.0)
+    assert lib().nh_paged_attention(C.byref(dev.kv), C.byref(rows), P(qd), n_head, scale, window, sinks, P(out),
+                                    _stream()) == 0
+    return out.cpu().numpy().reshape(q.shape)
+
+
+def _seen(pos, total, window, sinks):
+    t = np.arange(total)
+    return (t <= pos) & ((window == 0) | (t > pos - window) | (t < sinks))
+
+
+# Rows and heads a KV head that take each form: 2, 4, 8 and 16 queries a CTA, tiles.
+FORMS = [(2, 1), (2, 2), (5, 1), (8, 2), (80, 2), (200, 1)]
+
+
+@pytest.mark.parametrize("rows_n,group", FORMS)
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("case", ["later pages", "earlier pages", "no numbers"])
+def test_hidden_scales_do_not_count(gpu, rows_n, group, hd, case):
+    """V's scale grows by many powers of two from page to page where causality hides the later pages from a row, or falls where the
+    window hides the earlier ones, or is not a number there: each row is held to the largest value that it sees itself."""
+    n_kv, page = 2, 16
+    p0 = {"later pages": page - 1, "earlier pages": 60, "no numbers": page - 1}[case]
+    window = 20 if case == "earlier pages" else 0
+    total = p0 + rows_n
+    rng, table, cache, dev = _setup([rows_n], [p0], group * n_kv, n_kv, hd, page, rows_n + hd)
+    blocks = (total + page - 1) // page
+    for b in range(blocks):
+        pg = table[0, b]
+        step = 200 // blocks
+        e = -100 + step * b if case != "earlier pages" else 100 - step * b
+        cache.scales[1][pg] = 1.0 if case == "no numbers" else 2.0 ** e
+        if case == "no numbers" and b > 0:
+            cache.scales[0][pg], cache.scales[1][pg] = [np.nan, np.inf], [np.inf, np.nan]
+    for w in range(2):
+        dev.scales[w].copy_(_cuda(cache.scales[w]))
+    q = rng.standard_normal((rows_n, group * n_kv, hd)).astype(np.float32)
+    got = _attend(dev, q, [rows_n], [p0], group * n_kv, 0.125, window, 0)
+    clean = cache.copy()
+    for w in range(2):
+        clean.scales[w][~np.isfinite(clean.scales[w])] = 1.0
+    k, v = clean.values(0, table[0], total), clean.values(1, table[0], total)
+    want, size = pm.attention(q, k, v, p0, 0.125, window, 0)
+    for i in range(rows_n):
+        sel = _seen(p0 + i, total, window, 0)
+        if case == "no numbers" and p0 + i >= page:
+            break
+        bound = pm.attention_bound(size, hd, total, np.abs(v[sel]).max())
+        assert np.abs(got[i] - want[i]).max() <= bound, i

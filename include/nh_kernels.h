@@ -459,8 +459,9 @@ typedef struct NhPagedKv {
  * outside those bounds or past max_blocks pages, and a page outside
  * [0, n_pages), are not touched and record NH_E_ARG in *err (err may be null):
  * such a sequence's rows are left as they were, such a page's positions are
- * neither written nor seen.  Rows at and after row_off[n_seq] are left as they
- * were.  A page that is written belongs to one sequence of the call; pages
+ * neither written nor seen.  A page of which no row of the call sees or writes
+ * a position (behind the window, past the last row) may have any entry.  Rows
+ * at and after row_off[n_seq] are left as they were.  A page that is written belongs to one sequence of the call; pages
  * that are only read may be shared. */
 typedef struct NhPagedRows {
   int32_t n_seq;      /* 1 .. 65535 */

@@ -303,13 +303,14 @@ __global__ void __launch_bounds__(kTileThreads, 1) paged_tile_kernel(const Paged
     const uint32_t page_bytes = static_cast<uint32_t>(p.kv.n_kv) * static_cast<uint32_t>(page * HD);  // at most 2^30
     const int32_t* table = p.rows.page_table + static_cast<int64_t>(s) * p.rows.max_blocks;
     // Pages of this warp's two 16-position parts of 16 tiles: lane l has part l & 1 of tile f + (l >> 1).  -1: none (past
-    // the last position), -2: out of range.
+    // the last position, or between the sinks and the window of every query: its page may have been given up), -2: out
+    // of range.
     auto ids_of = [&](int f) {
       const int j = f + (lane >> 1);
       int id = -1;
       if (j < n) {
         const int t = tile_pos(j) + w * 32 + (lane & 1) * kSub;
-        if (t <= last_pos) {
+        if (t <= last_pos && (p.window == 0 || t + kSub - 1 > first_pos - p.window || t < p.n_sink)) {
           id = __ldcg(table + (t >> lg));
           if (id < 0 || id >= p.kv.n_pages) id = -2;
         }

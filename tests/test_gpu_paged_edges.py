@@ -9,7 +9,7 @@ import pytest
 
 from nuthatch_b200._lib import lib
 from tests import paged_model as pm
-from tests.test_gpu_paged import P, _cuda, _setup, _stream
+from tests.test_gpu_paged import NH_E_ARG, P, _cuda, _setup, _stream
 
 pytestmark = pytest.mark.gpu
 
@@ -68,3 +68,26 @@ def test_hidden_scales_do_not_count(gpu, rows_n, group, hd, case):
             break
         bound = pm.attention_bound(size, hd, total, np.abs(v[sel]).max())
         assert np.abs(got[i] - want[i]).max() <= bound, i
+
+
+@pytest.mark.parametrize("n_head", [2, 4])
+def test_pages_behind_the_window_may_be_gone(gpu, n_head):
+    """A sequence that gives up its pages between the sinks and the window: nothing is reported, nothing missed."""
+    n_kv, hd, page, window, sinks = 2, 64, 16, 50, 4
+    for rows_n in (1, 3, 9, 120):
+        p0 = 307
+        total = p0 + rows_n
+        rng, table, cache, dev = _setup([rows_n], [p0], n_head, n_kv, hd, page, rows_n)
+        first = (p0 - window + 1) // page  # the page of the first position that the first row's window holds
+        for b in range(1, first):
+            dev.table[0, b] = -1 if b % 2 else 1 << 29
+        q = rng.standard_normal((rows_n, n_head, hd)).astype(np.float32)
+        got = _attend(dev, q, [rows_n], [p0], n_head, 0.125, window, sinks)
+        assert int(dev.err.item()) == 0, rows_n
+        k, v = cache.values(0, table[0], total), cache.values(1, table[0], total)
+        want, size = pm.attention(q, k, v, p0, 0.125, window, sinks)
+        assert np.abs(got - want).max() <= pm.attention_bound(size, hd, total, np.abs(v).max())
+        # one page more is missed
+        dev.table[0, first] = -1
+        _attend(dev, q, [rows_n], [p0], n_head, 0.125, window, sinks)
+        assert int(dev.err.item()) == NH_E_ARG, rows_n

@@ -546,7 +546,7 @@ __device__ __forceinline__ void split_queries(const PagedAttnArgs& p) {
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
         const float v = kSmall ? o[n][2 * e] + o[n][2 * e + 1] : NQ == 8 ? o[n][e] + o[n][e + 2] : o[n][2 * k + e];
-        sh.o[warp][qk][kSmall ? (2 * n + e) * 8 + g : n * 8 + 2 * t + e] = v * pow2i(kCodeShift - kWeightShift) * unit;
+        sh.o[warp][qk][kSmall ? (2 * n + e) * 8 + g : n * 8 + 2 * t + e] = v * pow2i(kCodeShift - kWeightShift - kRoom) * unit;
       }
   }
   __syncthreads();
@@ -585,7 +585,7 @@ __device__ __forceinline__ void split_queries(const PagedAttnArgs& p) {
       v += a * cluster.map_shared_rank(&sh.o[0][q][0], r)[place];
     }
     const int row = sq.r0 + qi / p.group, head = kh * p.group + qi % p.group;
-    p.out[(static_cast<int64_t>(row) * p.n_head + head) * HD + d] = sum == 0.f ? 0.f : v / sum;
+    p.out[(static_cast<int64_t>(row) * p.n_head + head) * HD + d] = sum == 0.f ? 0.f : v / sum * pow2i(kRoom);
   }
   if (nrank > 1) cluster.sync();  // no CTA leaves while another reads its part
 }

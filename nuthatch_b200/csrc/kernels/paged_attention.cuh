@@ -26,6 +26,11 @@ struct PagedAttnArgs {
 constexpr float kLog2e = 1.44269504088896340736f;
 constexpr int kWeightShift = 15;  // a weight in [0, 1] times 2^15 keeps 22 bits in two f16 parts down to 2^-29
 
+// Sums of weighted values in their own units pass f32's range where the values are near its end, and their mean does
+// not: what is joined over warps and CTAs is smaller by 2^18 (2^18 positions of equal weight and the largest values; the
+// least scale, 2^-106, keeps its 24 bits above the subnormals).
+constexpr int kRoom = 18;
+
 // 2^e as a float, 0 below the normal range; e <= 127.
 __device__ __forceinline__ float pow2i(int e) { return e < -126 ? 0.f : __int_as_float((e + 127) << 23); }
 __device__ __forceinline__ int exponent_of(float s) { return ((__float_as_int(s) >> 23) & 255) - 127; }

@@ -757,7 +757,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) paged_tile_kernel(const Paged
       const float2 at = n > kFlush ? sh.at_flush[row] : last;
       add_sums(half * (HD / 32), (half + 1) * (HD / 32), n > kFlush,
                factor(at.x, last.x) * pow2i(max(__float_as_int(at.y) - __float_as_int(last.y), -200)), 1.f,
-               [=](float x) { return x * (pow2i(kCodeShift - kTileShift) * unit) * inv; });
+               [=](float x) { return x * inv * (pow2i(kCodeShift - kTileShift - (nrank > 1 ? kRoom : 0)) * unit); });
     }
     tc_before();
   }
@@ -790,7 +790,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) paged_tile_kernel(const Paged
           v.z += a * y.z;
           v.w += a * y.w;
         }
-        const float inv = sum == 0.f ? 0.f : 1.f / sum;
+        const float inv = sum == 0.f ? 0.f : 1.f / sum * pow2i(kRoom);
         reinterpret_cast<float4*>(p.out + sh.row_at[row])[d] = make_float4(v.x * inv, v.y * inv, v.z * inv, v.w * inv);
       }
     }

@@ -91,3 +91,21 @@ def test_pages_behind_the_window_may_be_gone(gpu, n_head):
         dev.table[0, first] = -1
         _attend(dev, q, [rows_n], [p0], n_head, 0.125, window, sinks)
         assert int(dev.err.item()) == NH_E_ARG, rows_n
+
+
+@pytest.mark.parametrize("rows_n,group", FORMS)
+def test_largest_values(gpu, rows_n, group):
+    """Values up to f32's range: the sum of the weighted values passes it, their mean does not."""
+    n_kv, hd, page = 2, 64, 16
+    for p0 in (100, 3000):
+        total = p0 + rows_n
+        rng, table, cache, dev = _setup([rows_n], [p0], group * n_kv, n_kv, hd, page, rows_n)
+        cache.scales[1][:] = 2.0 ** 121
+        cache.codes[1][:] = np.where(rng.random(cache.codes[1].shape) < 0.9, 255, 0)
+        dev.scales[1].copy_(_cuda(cache.scales[1]))
+        dev.codes[1].copy_(_cuda(cache.codes[1]))
+        q = rng.standard_normal((rows_n, group * n_kv, hd)).astype(np.float32)
+        got = _attend(dev, q, [rows_n], [p0], group * n_kv, 0.125, 0, 0).astype(np.float64)
+        k, v = cache.values(0, table[0], total), cache.values(1, table[0], total)
+        want, size = pm.attention(q, k, v, p0, 0.125, 0, 0)
+        assert np.abs(got - want).max() <= pm.attention_bound(size, hd, total, np.abs(v).max()), p0

@@ -56,13 +56,15 @@ __device__ __forceinline__ int scale_exponent(uint32_t amax_bits) {
 __device__ __forceinline__ float exponent_float(int biased) { return __int_as_float(biased << 23); }
 
 // floor(x * inv) + 128 in the low byte, for a finite x within the scale: the
-// sum with 1.5 * 2^23, rounded down, holds the floor in its low bits.
+// sum with 1.5 * 2^23, rounded down, holds the floor in its low bits.  (The
+// product is exact, or below the subnormals and rounded down too: a negative
+// x has floor -1 however small it is.)
 __device__ __forceinline__ uint32_t code_bits(float x, float inv) {
-  return __float_as_uint(__fadd_rd(__fmul_rn(x, inv), 12582912.f + 128.f));
+  return __float_as_uint(__fadd_rd(__fmul_rd(x, inv), 12582912.f + 128.f));
 }
 // The same for any x: the nearest end of the range, a NaN as its middle.
 __device__ __forceinline__ uint32_t code_of(float x, float inv) {
-  return static_cast<uint32_t>(min(max(__float2int_rd(x * inv), -128), 127) + 128);
+  return static_cast<uint32_t>(min(max(__float2int_rd(__fmul_rd(x, inv)), -128), 127) + 128);
 }
 
 // Warps a head, rows a warp and threads for a page size.

@@ -9,7 +9,7 @@ import pytest
 
 from nuthatch_b200._lib import lib
 from tests import paged_model as pm
-from tests.test_gpu_paged import NH_E_ARG, P, _cuda, _setup, _stream
+from tests.test_gpu_paged import NH_E_ARG, P, _append, _cuda, _same_cache, _setup, _stream
 
 pytestmark = pytest.mark.gpu
 
@@ -109,3 +109,29 @@ def test_largest_values(gpu, rows_n, group):
         k, v = cache.values(0, table[0], total), cache.values(1, table[0], total)
         want, size = pm.attention(q, k, v, p0, 0.125, 0, 0)
         assert np.abs(got - want).max() <= pm.attention_bound(size, hd, total, np.abs(v).max()), p0
+
+
+@pytest.mark.parametrize("hd,page", [(32, 16), (64, 32), (96, 128), (128, 64)])
+def test_codes_of_tiny_values_under_large_scales(gpu, hd, page):
+    """floor(x / scale) of a negative x is -1 however small x is, in one call or over several."""
+    n_kv, n = 2, 9
+    rng, table, cache, dev = _setup([n], [0], n_kv, n_kv, hd, page, 4)
+    _, _, _, dev2 = _setup([n], [0], n_kv, n_kv, hd, page, 4)
+    v = (-np.exp2(rng.uniform(-148, 60, (n, n_kv, hd)))).astype(np.float32)
+    v[:, :, ::3] *= -1
+    v[:, :, ::5] = 0.0
+    v[n - 1, 0, 1], v[n - 2, 1, 2] = 3.3e38, -2.0 ** 100
+    k = v[::-1].copy()
+    cs = np.zeros((n + 1, hd // 2, 2), np.float32)
+    cs[:, :, 0] = 1.0  # no rotation: K's rows are coded as they are
+    want = cache.copy()
+    for w, x in enumerate((k, v)):
+        want.append(w, table[0], 0, x)
+    kd, vd, cs = _cuda(k.reshape(n, -1)), _cuda(v.reshape(n, -1)), _cuda(cs)
+    rc, keep = _append(dev, [n], [0], None, kd, vd, None, None, cs, n_kv, None)
+    assert rc == 0 and int(dev.err.item()) == 0
+    _same_cache(dev.host(), want)
+    for at in range(n):
+        rc, keep = _append(dev2, [1], [at], None, kd[at:], vd[at:], None, None, cs, n_kv, None)
+        assert rc == 0
+    _same_cache(dev2.host(), want)

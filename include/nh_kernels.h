@@ -520,12 +520,14 @@ int nh_paged_read(const NhPagedKv* kv, const NhPagedRows* rows, int32_t out_type
  * target row.  The draw is the lowest id whose running sum exceeds
  * u_pick[s] * the sum.  draft null: the drafts are certain (probability 1 at
  * the drafted id, 0 elsewhere).  Products and sums are in 64 bits; an entry
- * that is not above 0 (a NaN too) has no mass.  Rows need not sum to 1.
+ * that is not above 0 (a NaN too) has no mass, an infinite draft entry leaves
+ * none of its id's.  Rows need not sum to 1.
  *   n_accept [n_seq]; out_ids [n_seq][max_draft+1]: the accepted ids, then the
  *   drawn one; what follows is left as it was.
- * A draft id outside [0, n_vocab) is refused; a row without mass draws id -1;
- * both record NH_E_ARG in *err (may be null).  So does a sequence with n < 0 or
- * n > max_draft or an offset outside [0, n_drafts]; nothing is written for it.
+ * A draft id outside [0, n_vocab) is refused; a row without mass, or of infinite
+ * mass, draws id -1; both record NH_E_ARG in *err (may be null).  So does a
+ * sequence with n < 0 or n > max_draft or an offset outside [0, n_drafts];
+ * nothing is written for it.
  * Every row is at most 2^30 ids long. */
 typedef struct NhVerifyDrafts {
   const float* target;    /* [n_drafts + n_seq] rows */

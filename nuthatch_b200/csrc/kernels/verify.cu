@@ -44,12 +44,12 @@ struct Source {
   bool vec;        // both rows are 16-byte aligned
 };
 
-// A piece of four masses: p less q where that is above 0.
+// A piece of four masses: p less q where that is above 0 (an infinite q leaves nothing).
 __device__ __forceinline__ void masses(const float4& p, const float4& q, double (&m)[4]) {
   const float b[4] = {mass(q.x), mass(q.y), mass(q.z), mass(q.w)};
-  const float a[4] = {fmaxf(p.x, b[0]), fmaxf(p.y, b[1]), fmaxf(p.z, b[2]), fmaxf(p.w, b[3])};
+  const float a[4] = {p.x, p.y, p.z, p.w};
 #pragma unroll
-  for (int j = 0; j < 4; ++j) m[j] = static_cast<double>(a[j]) - static_cast<double>(b[j]);
+  for (int j = 0; j < 4; ++j) m[j] = a[j] > b[j] ? static_cast<double>(a[j]) - static_cast<double>(b[j]) : 0.0;
 }
 __device__ __forceinline__ void masses(const float4& p, double (&m)[4]) {
   m[0] = static_cast<double>(mass(p.x));
@@ -213,7 +213,8 @@ __global__ void __launch_bounds__(kVerifyThreads) verify_drafts_kernel(const NhV
 
   const double goal = static_cast<double>(u_pick) * all;
   double before = 0.0;
-  const int owner = find_part(lane < nrank ? total[pass][lane] : 0.0, nrank, goal, lane, before);
+  int owner = find_part(lane < nrank ? total[pass][lane] : 0.0, nrank, goal, lane, before);
+  if (all == INFINITY) owner = -1;  // an infinite entry of the target: no distribution
   int32_t* ids = d.out_ids + static_cast<int64_t>(s) * (d.max_draft + 1);
   if (rank == 0) {
     for (int i = tid; i < acc; i += kVerifyThreads) ids[i] = d.draft_ids[o + i];

@@ -9,7 +9,7 @@ import pytest
 
 from nuthatch_b200._lib import lib
 from tests import paged_model as pm
-from tests.test_gpu_paged import NH_E_ARG, P, _append, _cuda, _same_cache, _setup, _stream
+from tests.test_gpu_paged import NH_E_ARG, P, _append, _cuda, _probs, _same_cache, _setup, _stream, _verify_call
 
 pytestmark = pytest.mark.gpu
 
@@ -135,3 +135,27 @@ def test_codes_of_tiny_values_under_large_scales(gpu, hd, page):
         rc, keep = _append(dev2, [1], [at], None, kd[at:], vd[at:], None, None, cs, n_kv, None)
         assert rc == 0
     _same_cache(dev2.host(), want)
+
+
+def test_verify_infinite_entries(gpu):
+    """An infinite draft entry takes its own id's mass alone; a target row with an infinite one has no distribution."""
+    v, n = 700, 4
+    rng = np.random.default_rng(2)
+    off = np.arange(0, n + 1)
+    target, draft = _probs(rng, 2 * n, v, 1.0), _probs(rng, n, v, 1.0)
+    ids = np.array([3, 4, 5, 6])
+    for s in range(n):
+        draft[s, ids[s]] = 1.0
+    draft[0, [3, 9, 300]] = np.inf
+    draft[1, 4] = np.inf
+    draft[1, 650] = -np.inf      # not above 0: no mass
+    draft[2, :] = np.inf         # nothing is left: the target's own mass
+    target[2 * 3, 8] = np.inf    # the row that sequence 3's draw is from
+    ua, up = np.full(n, 0.9, np.float32), np.array([0.2, 0.7, 0.5, 0.5], np.float32)
+    acc, out, err = _verify_call(target, draft, ids, off, ua, up)
+    want_acc, want = pm.verify(target, draft, ids, off, ua, up)
+    assert list(acc) == [0, 0, 0, 0] == want_acc
+    assert [int(out[s, 0]) for s in range(3)] == [want[s][0] for s in range(3)]
+    assert int(out[3, 0]) == -1 and err == NH_E_ARG
+    acc, out, err = _verify_call(target[:6], draft[:3], ids[:3], off[:4], ua[:3], up[:3])
+    assert err == 0 and [int(out[s, 0]) for s in range(3)] == [want[s][0] for s in range(3)]

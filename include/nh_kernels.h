@@ -494,7 +494,7 @@ int nh_paged_append(const NhPagedKv* kv, const NhPagedRows* rows, const float* q
  * the positions t <= p of a row at position p with, when window > 0,
  * t > p - window or t < n_sink (the window's positions and the first n_sink,
  * which stay visible).  qr and out are [n_rows][n_head*head_dim], 16-byte
- * aligned; any n_head that n_head_kv divides.  No scratch: a sequence with few
+ * aligned; any n_head that n_head_kv divides; kq_scale is finite.  No scratch: a sequence with few
  * rows is split over the CTAs of a cluster, joined in a fixed order, so equal
  * calls give equal bits.  A row that sees no position gives zeros.  max_rows *
  * n_head / n_head_kv is below 2^31. */

@@ -28,6 +28,7 @@
 //   conversion shared by twice the queries.
 #include <cooperative_groups.h>
 
+#include <cmath>
 #include <cstddef>
 
 #include "paged_attention.cuh"
@@ -673,7 +674,7 @@ extern "C" int nh_paged_attention(const NhPagedKv* kv, const NhPagedRows* rows, 
   const int rc = paged_args(kv, rows, p.kv, p.rows);
   if (rc != NH_OK) return rc;
   if (qr == nullptr || out == nullptr || !paged_aligned(qr) || !paged_aligned(out) || n_head <= 0 || n_head > 65535 ||
-      n_head % p.kv.n_kv != 0 || window < 0 || n_sink < 0 ||
+      n_head % p.kv.n_kv != 0 || window < 0 || n_sink < 0 || !std::isfinite(kq_scale) ||
       static_cast<int64_t>(p.rows.max_rows) * (n_head / p.kv.n_kv) > INT32_MAX)  // queries are counted in 32 bits
     return NH_E_ARG;
   if (p.rows.max_rows == 0) return NH_OK;

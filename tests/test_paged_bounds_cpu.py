@@ -1,0 +1,13 @@
+"""Values of the paged-cache entries' arguments that would give no result: refused
+calls launch nothing, so they need no GPU."""
+from __future__ import annotations
+
+import pytest
+
+from tests.test_paged_refusals_cpu import NH_E_ARG, _attention, _kv, _rows
+
+
+@pytest.mark.parametrize("scale", [float("nan"), float("inf"), -float("inf")])
+def test_attention_factor_is_finite(scale):
+    assert _attention(_kv(), _rows(), scale=scale) == NH_E_ARG
+    assert _attention(_kv(), _rows(n_rows=0), scale=scale) == NH_E_ARG

@@ -736,12 +736,15 @@ __global__ void __launch_bounds__(kTileThreads, 1) paged_tile_kernel(const Paged
     }
     if (n > 0 && ok) ok = products_done(n - 1);
     if (__any_sync(0xffffffffu, !ok) && lane == 0) sh.failed = 1;
-    // Every product is done: the row's values in their own units.
+    // Every product is done: the row's values in their own units.  The group that did not take the last tile may not
+    // have seen the phase before the one that it has waited for, whose parity then lets it through at once; the other
+    // group's wait is sure, so the reads of O come after the barrier of both and a fence behind it.
     __syncwarp();
-    tc_after();
     sh.l[half][row] = row_l;
     sh.lm[half][row] = row_m;
+    tc_before();
     asm volatile("bar.sync 1, 256;\n" ::: "memory");
+    tc_after();
     const float2 last = n > 0 && !idle ? sh.ref[(n - 1) & 1][row] : make_float2(-INFINITY, __int_as_float(-200));
     const float unit = pow2i(max(__float_as_int(last.y), -126));
     const float l = sh.l[0][row] * factor(sh.lm[0][row], last.x) + sh.l[1][row] * factor(sh.lm[1][row], last.x);

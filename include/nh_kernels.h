@@ -15,7 +15,8 @@
  *
  * Kernels taking an NhDecodeState* record a failed bounded device-side wait
  * as NH_E_TIMEOUT in state->error (the state may be NULL for the standalone
- * forms, which then only stop early).
+ * forms, which then only stop early).  nh_paged_attention records it in
+ * NhPagedRows.err and gives NaN in the rows concerned.
  *
  * Activations that meet a quantised weight are quantised to Q8_K inside the
  * kernel exactly as ggml's CPU mul_mat does (per 256 values: the element of
@@ -44,7 +45,7 @@ extern "C" {
 #define NH_E_STATE (-5)       /* object in the wrong state (host API) */
 #define NH_E_NOMEM (-6)       /* device or host allocation failed (host API) */
 #define NH_E_CAPACITY (-7)    /* request beyond a stated capacity */
-#define NH_E_TIMEOUT (-8)     /* a bounded device-side wait expired (recorded in NhDecodeState.error) */
+#define NH_E_TIMEOUT (-8)     /* a bounded device-side wait expired (recorded in NhDecodeState.error, NhPagedRows.err) */
 
 /* Per-sequence decode cursor, resident in device memory.  The kernels read
  * `pos` (tokens already in the KV cache); nh_lm_head_argmax advances it, so a
@@ -496,7 +497,9 @@ int nh_paged_append(const NhPagedKv* kv, const NhPagedRows* rows, const float* q
  * which stay visible).  qr and out are [n_rows][n_head*head_dim], 16-byte
  * aligned; any n_head that n_head_kv divides; kq_scale is finite.  No scratch: a sequence with few
  * rows is split over the CTAs of a cluster, joined in a fixed order, so equal
- * calls give equal bits.  A row that sees no position gives zeros.  max_rows *
+ * calls give equal bits.  A row that sees no position gives zeros.  A
+ * bounded wait inside the kernel that expires makes its rows NaN and records
+ * NH_E_TIMEOUT in *err (where no other code stands there yet).  max_rows *
  * n_head / n_head_kv is below 2^31. */
 int nh_paged_attention(const NhPagedKv* kv, const NhPagedRows* rows, const float* qr, int n_head, float kq_scale,
                        int window, int n_sink, float* out, void* stream);

@@ -38,7 +38,7 @@
 // leave tensor memory and are added up in shared memory, rounded.  (Every third:
 // 1.1e-6 against the f32 formula's 1.4e-6 on 2,048 rows after 2,048 others;
 // every seventh would save 5% of the time at 2.1e-6.)
-// All waits are bounded; an expired one records NH_E_TIMEOUT.
+// All waits are bounded; an expired one records NH_E_TIMEOUT and makes the rows NaN.
 #include <cooperative_groups.h>
 
 #include "paged_attention.cuh"
@@ -735,12 +735,13 @@ __global__ void __launch_bounds__(kTileThreads, 1) paged_tile_kernel(const Paged
       if (lane == 0) mbar_arrive(&sh.p_full[j % kScoreTiles]);
     }
     if (n > 0 && ok) ok = products_done(n - 1);
-    if (__any_sync(0xffffffffu, !ok) && lane == 0) sh.failed = 1;
+    const bool expired = __any_sync(0xffffffffu, !ok) != 0;
+    if (expired && lane == 0) sh.failed = 1;
     // Every product is done: the row's values in their own units.  The group that did not take the last tile may not
     // have seen the phase before the one that it has waited for, whose parity then lets it through at once; the other
     // group's wait is sure, so the reads of O come after the barrier of both and a fence behind it.
     __syncwarp();
-    sh.l[half][row] = row_l;
+    sh.l[half][row] = expired ? __int_as_float(0x7fc00000) : row_l;  // no number is taken for a result after an expired wait
     sh.lm[half][row] = row_m;
     tc_before();
     asm volatile("bar.sync 1, 256;\n" ::: "memory");

@@ -120,23 +120,41 @@ int launch_pdl(void (*kern)(KArgs...), dim3 grid, dim3 block, size_t smem, cudaS
   return cudaLaunchKernelEx(&cfg, kern, std::forward<Args>(args)...) == cudaSuccess ? NH_OK : NH_E_CUDA;
 }
 
-// Whether one kernel may be launched in clusters of 16 (above the portable 8),
-// set once per device as SmemLimit is.
+// Whether one kernel can be launched in clusters of 16 (above the portable 8),
+// asked once per device: 0 unknown, 1 yes, 2 no.
 struct WideCluster {
-  std::atomic<bool> set[SmemLimit::kMaxDevices];
+  std::atomic<int> can[SmemLimit::kMaxDevices];
   WideCluster() {
-    for (auto& s : set) s.store(false, std::memory_order_relaxed);
+    for (auto& c : can) c.store(0, std::memory_order_relaxed);
   }
 };
 
+// False where the device (or the part of it that the process has) cannot place
+// such a cluster with `smem` bytes a CTA, set for the kernel before; the caller
+// then takes eight.
 template <typename Kern>
-bool ensure_wide_cluster(Kern k, WideCluster& rec) {
+bool ensure_wide_cluster(Kern k, dim3 block, size_t smem, WideCluster& rec) {
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= SmemLimit::kMaxDevices) return false;
-  if (rec.set[dev].load(std::memory_order_acquire)) return true;
-  if (cudaFuncSetAttribute(k, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) != cudaSuccess) return false;
-  rec.set[dev].store(true, std::memory_order_release);
-  return true;
+  const int known = rec.can[dev].load(std::memory_order_acquire);
+  if (known != 0) return known == 1;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(16);
+  cfg.blockDim = block;
+  cfg.dynamicSmemBytes = smem;
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeClusterDimension;
+  at[0].val.clusterDim.x = 16;
+  at[0].val.clusterDim.y = 1;
+  at[0].val.clusterDim.z = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = 1;
+  int n = 0;
+  const bool can = cudaFuncSetAttribute(k, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) == cudaSuccess &&
+                   cudaOccupancyMaxActiveClusters(&n, k, &cfg) == cudaSuccess && n > 0;
+  if (!can) cudaGetLastError();  // the refusal is answered here
+  rec.can[dev].store(can ? 1 : 2, std::memory_order_release);
+  return can;
 }
 
 // launch_pdl with thread-block clusters of `cluster` CTAs along x.

@@ -608,13 +608,13 @@ template <int HD, int NQ>
 int launch_split(const PagedAttnArgs& p, int groups, int ranks, cudaStream_t s) {
   static SmemLimit configured;
   static WideCluster wide;
-  size_t smem = sizeof(SplitShared<HD, NQ>);
+  constexpr size_t kSmem = sizeof(SplitShared<HD, NQ>), kApart = NQ == 16 && kSmem < 76 * 1024 ? 76 * 1024 : kSmem;
+  if (!ensure_smem(paged_split_kernel<HD, NQ>, kApart, configured)) return NH_E_CUDA;
+  if (ranks > 8 && !ensure_wide_cluster(paged_split_kernel<HD, NQ>, dim3(kWarpsOf<NQ> * 32), kApart, wide)) ranks = 8;
   // Few CTAs are spread out: two to an SM where that holds them all (32 queries over 8,000 positions, 16 heads: 35 us,
   // with three to an SM 41).
-  if (NQ == 16 && static_cast<int64_t>(ranks) * p.kv.n_kv * groups * p.rows.n_seq <= 2 * device_sm_count())
-    smem = std::max<size_t>(smem, 76 * 1024);
-  if (!ensure_smem(paged_split_kernel<HD, NQ>, smem, configured)) return NH_E_CUDA;
-  if (ranks > 8 && !ensure_wide_cluster(paged_split_kernel<HD, NQ>, wide)) return NH_E_CUDA;
+  const bool apart = static_cast<int64_t>(ranks) * p.kv.n_kv * groups * p.rows.n_seq <= 2 * device_sm_count();
+  const size_t smem = apart ? kApart : kSmem;
   return launch_cluster(paged_split_kernel<HD, NQ>, dim3(ranks, p.kv.n_kv * groups, p.rows.n_seq),
                         dim3(kWarpsOf<NQ> * 32), ranks, smem, s, p);
 }

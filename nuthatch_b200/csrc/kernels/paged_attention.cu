@@ -422,7 +422,10 @@ __device__ __forceinline__ void split_queries(const PagedAttnArgs& p) {
                                   : c[e >> 1][2 * k + (e & 1)];
         x[k][e] = (NQ == 2 ? d + nan_q : d) * f;
       }
+      ev[k] = exponent_of(v_scale);
       if (!plain) {
+        if (!seen_here || t0 > pos[k] || (p.window != 0 && t0 + kUnit - 1 <= pos[k] - p.window && t0 >= p.n_sink))
+          ev[k] = eref[k];
 #pragma unroll
         for (int e = 0; e < ST; ++e) {
           const int tk = t0 + (kSmall ? g + 8 * e : 8 * (e >> 1) + 2 * t + (e & 1));
@@ -436,9 +439,6 @@ __device__ __forceinline__ void split_queries(const PagedAttnArgs& p) {
 #pragma unroll
       for (int e = kSmall ? 4 : 1; e <= (kSmall ? 16 : 2); e <<= 1)
         top[k] = fmaxf(top[k], __shfl_xor_sync(0xffffffffu, top[k], e));
-      const bool sees = plain || (seen_here && t0 <= pos[k] &&
-                                  (p.window == 0 || t0 + kUnit - 1 > pos[k] - p.window || t0 < p.n_sink));
-      ev[k] = sees ? exponent_of(v_scale) : eref[k];
       grew |= top[k] > m[k] || ev[k] > eref[k];
     }
     // Rarely after the first units: a larger score, or a larger scale of V.

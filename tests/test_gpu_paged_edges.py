@@ -159,3 +159,49 @@ def test_verify_infinite_entries(gpu):
     assert int(out[3, 0]) == -1 and err == NH_E_ARG
     acc, out, err = _verify_call(target[:6], draft[:3], ids[:3], off[:4], ua[:3], up[:3])
     assert err == 0 and [int(out[s, 0]) for s in range(3)] == [want[s][0] for s in range(3)]
+
+
+@pytest.mark.parametrize("n,p0", [([1, 1, 1], [20, 0, 333]), ([4, 2, 0], [20, 0, 333]), ([90, 1, 40], [0, 500, 30])])
+def test_rows_amid_larger_buffers(gpu, n, p0):
+    """Offsets that do not begin at 0, and bounds (rows, rows of a sequence, pages of the table) far above what the call
+    holds, as a captured step's are: the same rows and cache, the rest of the buffers left as it was."""
+    import torch
+
+    n_head, n_kv, hd, page, lead, behind = 8, 4, 64, 16, 3, 2000
+    R, dq, dkv = sum(n), n_head * hd, n_kv * hd
+    cs = _cuda(pm.rope_table(hd, 700))
+    got = []
+    for wide in (False, True):
+        rng, table, cache, dev = _setup(n, p0, n_head, n_kv, hd, page, 6)
+        if wide:
+            dev = pm.Device(cache, np.concatenate([table, np.full((len(n), 900), -1)], 1))
+        a, b = (lead, lead + R + behind) if wide else (0, R)
+        bufs = [torch.full((b, w), 7.0, device="cuda") for w in (dq, dkv, dkv, dq, dq, dkv, dkv)]
+        q, k, v, qr, out, ko, vo = bufs
+        for x in (q, k, v):
+            x[a:a + R] = _cuda(rng.standard_normal((R, x.shape[1])).astype(np.float32))
+        more = dict(max_rows=4000, n_rows=b, offset=lead) if wide else {}
+        rc, keep = _append(dev, n, p0, q, k, v, None, None, cs, n_head, qr, **more)
+        assert rc == 0
+        rows, keep2 = dev.rows(n, p0, **more)
+        assert lib().nh_paged_attention(C.byref(dev.kv), C.byref(rows), P(qr), n_head, 0.125, 0, 0, P(out), _stream()) == 0
+        assert lib().nh_paged_read(C.byref(dev.kv), C.byref(rows), 0, P(ko), P(vo), _stream()) == 0
+        assert int(dev.err.item()) == 0
+        for x in bufs[3:]:
+            assert (x[:a] == 7.0).all() and (x[a + R:] == 7.0).all()
+        h = dev.host()
+        got.append((qr[a:a + R], ko[a:a + R], vo[a:a + R], out[a:a + R], h))
+    for x, y in zip(got[0][:3], got[1][:3]):
+        assert torch.equal(x, y)
+    _same_cache(got[1][4], got[0][4])
+    at = 0
+    for s, m in enumerate(n):
+        if m:
+            total = m + p0[s]
+            k, v = got[0][4].values(0, table[s], total), got[0][4].values(1, table[s], total)
+            qs = got[0][0][at:at + m].cpu().numpy().reshape(m, n_head, hd)
+            want, size = pm.attention(qs, k, v, p0[s], 0.125, 0, 0)
+            for g in got:  # how the positions are shared out depends on the bounds, so the bits may differ
+                err = np.abs(g[3][at:at + m].cpu().numpy().reshape(want.shape) - want).max()
+                assert err <= pm.attention_bound(size, hd, total, np.abs(v).max())
+        at += m

@@ -456,7 +456,10 @@ typedef struct NhPagedKv {
  * is fine), at positions pos0[s], pos0[s]+1, ...; its position p lies in page
  * page_table[s*max_blocks + p / page_size].  The arrays are device memory and
  * may change between replays of a captured call; n_rows (rows of the row
- * buffers) and max_rows (most rows of one sequence) bound them.  A sequence
+ * buffers) and max_rows (most rows of one sequence) bound them.  The bounds
+ * steer the launches too: max_blocks stands for the longest sequence's length,
+ * and one far above it shares short sequences out over more CTAs than they
+ * need.  A sequence
  * outside those bounds or past max_blocks pages, and a page outside
  * [0, n_pages), are not touched and record NH_E_ARG in *err (err may be null):
  * such a sequence's rows are left as they were, such a page's positions are
@@ -477,15 +480,16 @@ typedef struct NhPagedRows {
 
 /* nh_prefill_qk for a paged cache: QK-norm over the full q and k width (with
  * q_norm and k_norm both null: none), NEOX RoPE at each row's position, the
- * rotated q into qr [n_rows][n_head*head_dim] (nh_prefill_qk's bits), and the
- * rotated K (worked out in 64 bits and rounded to f32 once) and raw V rows coded
- * into the cache.  Row r of q, k and v starts r * its stride floats in;
- * rope_cs is nh_rope_table's table of rope_len positions (a sequence past it
- * counts as out of bounds).  q and qr may both be null.  A K or V value that
- * is not finite is coded as the nearest end of the range (a NaN as its middle),
- * sets no scale, and records NH_E_ARG in *err.  Pointers are 16-byte aligned, strides
- * a multiple of 4 and at most 2^23; a call writes at most 65,535 pages of a
- * sequence. */
+ * rotated q into qr [n_rows][n_head*head_dim] (nh_prefill_qk's arithmetic; the
+ * 64-bit sum of squares is added up in an order of its own, which in rare cases
+ * rounds the row's factor to the neighbouring f32), and the rotated K (worked
+ * out in 64 bits and rounded to f32 once) and raw V rows coded into the cache.
+ * Row r of q, k and v starts r * its stride floats in; rope_cs is
+ * nh_rope_table's table of rope_len positions (a sequence past it counts as out
+ * of bounds).  q and qr may both be null.  A K or V value that is not finite is
+ * coded as the nearest end of the range (a NaN as its middle), sets no scale,
+ * and records NH_E_ARG in *err.  Pointers are 16-byte aligned, strides a multiple
+ * of 4 and at most 2^23; a call writes at most 65,535 pages of a sequence. */
 int nh_paged_append(const NhPagedKv* kv, const NhPagedRows* rows, const float* q, int64_t q_stride, const float* k,
                     int64_t k_stride, const float* v, int64_t v_stride, const float* q_norm, const float* k_norm,
                     float eps, int n_head, const float* rope_cs, int rope_len, float* qr, void* stream);
@@ -495,12 +499,16 @@ int nh_paged_append(const NhPagedKv* kv, const NhPagedRows* rows, const float* q
  * the positions t <= p of a row at position p with, when window > 0,
  * t > p - window or t < n_sink (the window's positions and the first n_sink,
  * which stay visible).  qr and out are [n_rows][n_head*head_dim], 16-byte
- * aligned; any n_head that n_head_kv divides; kq_scale is finite.  No scratch: a sequence with few
- * rows is split over the CTAs of a cluster, joined in a fixed order, so equal
- * calls give equal bits.  A row that sees no position gives zeros.  A
- * bounded wait inside the kernel that expires makes its rows NaN and records
- * NH_E_TIMEOUT in *err (where no other code stands there yet).  max_rows *
- * n_head / n_head_kv is below 2^31. */
+ * aligned; any n_head that n_head_kv divides; kq_scale is finite, its products
+ * with qr within f32's range.  Queries and weights go into the products as two
+ * f16 parts (or whole numbers of 23 bits), added up in f32; where a weight is too
+ * small for two parts, a result is off by at most 2^-32 of the largest magnitude
+ * of V that its row sees, for each such position.  No scratch: a sequence with
+ * few rows is split over the CTAs of a cluster, joined in a fixed order, so equal
+ * calls give equal bits.  A row that sees no position gives zeros.  A bounded
+ * wait inside the kernel that expires makes its rows NaN and records NH_E_TIMEOUT
+ * in *err (where no other code stands there yet).  max_rows * n_head / n_head_kv
+ * is below 2^31. */
 int nh_paged_attention(const NhPagedKv* kv, const NhPagedRows* rows, const float* qr, int n_head, float kq_scale,
                        int window, int n_sink, float* out, void* stream);
 

@@ -53,7 +53,8 @@ inline int paged_args(const NhPagedKv* kv, const NhPagedRows* rows, PagedKv& k, 
     return NH_E_ARG;
   if (kv->n_pages <= 0 || kv->n_head_kv <= 0 || kv->n_head_kv > 65535 || kv->head_dim <= 0 ||
       kv->head_dim % 32 != 0 || kv->head_dim > 128 ||
-      static_cast<int64_t>(kv->n_head_kv) * kv->page_size * kv->head_dim > (1 << 30) || !paged_aligned(kv->k_codes) || !paged_aligned(kv->v_codes))
+      static_cast<int64_t>(kv->n_head_kv) * kv->page_size * kv->head_dim > (1 << 30) || !paged_aligned(kv->k_codes) ||
+      !paged_aligned(kv->v_codes))
     return NH_E_ARG;
   int log2 = 4;
   while (log2 < 7 && (1 << log2) < kv->page_size) ++log2;

@@ -1,17 +1,10 @@
 // Attention over the paged 8-bit K/V cache for few rows a sequence: decode
 // positions and drafted ones (nh_paged_attention's split form).
 //
-// What bounds it: every cached byte is read once, so the copy rate of HBM; with
-// more queries the instructions of the codes' conversion and of the products'
-// operands.  Measured (16 KV heads of 128, one query each): 64 sequences of up
-// to 4,096 positions 128 us (5.4 TB/s of a copy's 6.5; the reads alone take 114,
-// unequal lengths on 296 places for CTAs), one of 131,001 positions 135 us
-// (4.0 TB/s: 256 CTAs on 148 SMs); 16 of up to 6,001, 8 heads of 128, 20 queries
-// each 78 us, 32 queries 93.  Measured and left: CTAs in order of length (129 us), two stages
-// and three CTAs to an SM (156), page ids fetched in the units' loop.  A CTA takes up to 2, 4, 8 or 16 queries of one (sequence, KV head) and a contiguous
-// part of the positions; a cluster's CTAs split the positions and join their
-// (maximum, sum, weighted values) through distributed shared memory in rank
-// order.  A warp takes units of 16 positions, always inside one page, through a
+// A CTA takes up to 2, 4, 8 or 16 queries of one (sequence, KV head) and a
+// contiguous part of the positions; a cluster's CTAs split the positions and
+// join their (maximum, sum, weighted values) through distributed shared memory
+// in rank order.  A warp takes units of 16 positions, always inside one page, through a
 // ring of stages of its own in shared memory (cp.async, no barrier between
 // warps), and reads them in the operand layout of mma.m16n8k16: both the
 // dimensions of K and those of V may be permuted freely, so each lane reads
@@ -26,6 +19,15 @@
 //   the codes are B; the score accumulators are the weights' operand layout.
 //   16 queries: two A operands (the query's wait in shared memory), the codes'
 //   conversion shared by twice the queries.
+// What bounds it: every cached byte is read once, so the copy rate of HBM; with
+// more queries the instructions of the codes' conversion and of the products'
+// operands.  Measured (16 KV heads of 128, one query each): 64 sequences of up
+// to 4,096 positions 127 us (5.4 TB/s of a copy's 6.5; the reads alone take 114,
+// unequal lengths on 296 places for CTAs), one of 131,001 positions 133 us
+// (4.0 TB/s: 256 CTAs on 148 SMs); 16 of up to 6,001, 8 heads of 128, 20 queries
+// each 78 us, 32 queries 93.  Measured and left: CTAs in order of length (129
+// us), two stages and three CTAs to an SM (156), page ids fetched in the units'
+// loop.
 #include <cooperative_groups.h>
 
 #include <cmath>
@@ -44,8 +46,8 @@ constexpr int kUnit = 16;  // positions of one warp step
 // the queries: 16 sequences of up to 6,001 positions, 8 KV heads of 128, take 93 us here and 129 tiled with 32 queries,
 // 130 and 130 with 48, 171 and 129 with 64; one of 8,000 positions and 16 KV heads 35 and 53 with 32.
 constexpr int kFewQueries = 32;
-// Warps of a CTA: sixteen to an SM either way by their registers, in fewer and larger CTAs for four queries (one long
-// sequence 158 -> 135 us, the decode batch 134 -> 127 us against four warps a CTA).
+// Warps of a CTA: sixteen to an SM either way by their registers, in fewer and larger CTAs for up to four queries (one
+// long sequence 158 -> 135 us, the decode batch 134 -> 127 us against four warps a CTA).
 template <int NQ>
 constexpr int kWarpsOf = NQ <= 4 ? 8 : 4;
 
@@ -625,7 +627,8 @@ int launch_split(const PagedAttnArgs& p, int groups, int ranks, cudaStream_t s) 
 // CTAs a group, 105 with 4, 114 with 4 and two CTAs to an SM; 20 queries: 88 with 2, 78 with 4.  More
 // are not free (each forms the query's operand and joins what it has), so a warp keeps a unit, and a cluster
 // larger than the portable eight, which is slow to start, has more: one sequence's 8,000 positions of 16 heads take
-// 17.6 us with 8 CTAs a head and 22.6 with 16, 131,001 positions 150 and 133.
+// 17.6 us with 8 CTAs a head and 22.6 with 16, 131,001 positions 150 and 133.  The length is taken to be the page
+// table's width, the only one that the host knows.
 template <int HD, int NQ>
 int launch_group(const PagedAttnArgs& p, int most, cudaStream_t s) {
   const int groups = (most + NQ - 1) / NQ, halves = 2 * groups - (NQ == 16 && most - (groups - 1) * NQ <= 8 ? 1 : 0);

@@ -6,6 +6,11 @@
 // (u - 127.5) * 2^-9 is exact in f16.  A query row is scaled by a power of two and
 // split into two f16 parts (22 bits of it), likewise a softmax weight; both
 // parts' products are exact and the tensor cores add them up in f32.
+// A weight carries its page's scale of V over the largest scale that its row
+// sees.  Of what that makes the two parts keep 22 bits down to 2^-18 of the
+// largest weight (split form; 2^-10 of the maximum in use in the tiled one);
+// below, f16's subnormals end, and the error is at most 2^-40 (2^-32): for each
+// position that part of the largest magnitude of V that the row sees.
 #pragma once
 
 #include "common.cuh"
@@ -24,7 +29,9 @@ struct PagedAttnArgs {
 };
 
 constexpr float kLog2e = 1.44269504088896340736f;
-constexpr int kWeightShift = 15;  // a weight in [0, 1] times 2^15 keeps 22 bits in two f16 parts down to 2^-29
+// A weight in [0, 1] times 2^15 is within f16's range; its second part ends at steps of 2^-24, so that the two keep 22
+// bits of weights of 2^-18 and more and are off by at most 2^-25 of the product, 2^-40 of the weight 1, below.
+constexpr int kWeightShift = 15;
 
 // Sums of weighted values in their own units pass f32's range where the values are near its end, and their mean does
 // not: what is joined over warps and CTAs is smaller by 2^18 (2^18 positions of equal weight and the largest values; the

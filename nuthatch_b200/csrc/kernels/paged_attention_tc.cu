@@ -15,18 +15,22 @@
 // What bounds it.  The products: f32 queries and weights as two f16 parts each
 // make 8 hd operations a score where one f16 pass would make 4, 2,048 cycles a
 // tile of 128 dimensions; the exponentials, 1,024 cycles a tile.  At present the
-// way of a tile from its scores to its weights is longer than either: some 5,000
-// cycles (tensor memory's loads, the exponentials, the hand-over), of which the
-// two groups of warps hide half, and 10,000 before a CTA's first tile.  2,048
-// rows after 2,048 others, 16 heads of 128: 124 us (half of the tensor cores'
-// measured rate with both parts counted); four prompts of up to 4,000 rows, 16
-// heads of 64 over 8, window 1,024: 240 us.  (Both groups on one tile, half of
-// its columns each: 137 and 274 us.  Walking a tile in loops instead of unrolled:
-// 129 and 251.  Narrow heads as two CTAs to an SM, each with one group of softmax
-// warps and one score tile, which would hide the starts: 253 us for 247, 91 for 76
-// with one prompt, as each tile then waits for its own products.  A CTA's start
-// is mostly its queries': 16 copies by each of eight warps 240 us, 32 by four
-// 245, 128 by one 281, 16-byte copies 253, loads into registers 248.)
+// way of a tile from its scores to its weights (tensor memory's loads, the
+// exponentials, the hand-over) is longer than either, although the two groups of
+// warps share it: 2.6 us a tile of 128 dimensions (5,100 cycles at 1,965 MHz),
+// 1.4 us (2,750) of 64, and some 12 us of a launch of one CTA to an SM belong to
+// none (nine sequences of 128 rows, 16 heads, 1 to 64 tiles each: 15 to 177 us,
+// 14 to 102 of 64 dimensions).  2,048 rows after 2,048 others, 16 heads of 128:
+// 123 us (half of the tensor cores' measured rate with both parts counted); four
+// prompts of up to 4,000 rows, 16 heads of 64 over 8, window 1,024: 244 us.
+// Measured and left, beside 125 and 240 to 247 us of the states they were tried in:
+// both groups on one tile, half of its columns each, 137 and 274; walking a tile
+// in loops instead of unrolled, 129 and 251; narrow heads as two CTAs to an SM,
+// each with one group of softmax warps and one score tile, which would hide the
+// starts, 253 for 247, and 91 for 76 with one prompt, as each tile then waits for
+// its own products.  A CTA's start is mostly its queries': 16 copies by each of
+// eight warps 240 us, 32 by four 245, 128 by one 281, 16-byte copies 253, loads
+// into registers 248.
 // Operand tiles lie in shared memory as rows of 64 dimensions, 128 bytes swizzled:
 // the same image serves K (K-major) and V (MN-major), and eight lanes write to
 // different banks.
@@ -37,7 +41,8 @@
 // sum towards zero (9e-6 of it at 4,096 positions): the sums of every few tiles
 // leave tensor memory and are added up in shared memory, rounded.  (Every third:
 // 1.1e-6 against the f32 formula's 1.4e-6 on 2,048 rows after 2,048 others;
-// every seventh would save 5% of the time at 2.1e-6.)
+// every seventh would save 5% of the time at 2.1e-6.  With values of one sign,
+// where nothing cancels what is cut off, 2.5e-6.)
 // All waits are bounded; an expired one records NH_E_TIMEOUT and makes the rows NaN.
 #include <cooperative_groups.h>
 
@@ -58,7 +63,7 @@ constexpr int kSoftThreads = 256;
 constexpr float kLeast = 1.17549435e-38f;  // factor of the scores at least: a hidden one, -inf, stays that
 constexpr int kHidden = -1000;     // V's exponent where no position is seen
 constexpr int kHalfBytes = kTileK * 128;  // 64 dimensions of an operand tile
-constexpr int kTileShift = 7;   // weights are 2^7 times [0, 2^8]
+constexpr int kTileShift = 7;   // weights are 2^7 times [0, 2^8], of the maximum in use: 22 bits of those from 2^-10 on
 constexpr int kFlush = 3;       // tiles whose products are added up in tensor memory
 constexpr int kScalePlaces = 8;
 constexpr int kLowest = -60;    // least power of two of a part's weights that products take
@@ -88,7 +93,8 @@ struct TileShared {
   float2 at_flush[kTileQ];   // the same, of the sums in `rows`
   float top[2][kTileQ];      // largest magnitudes of the query's halves
   int64_t row_at[kTileQ];  // where a query's row starts in q and out
-  uint64_t full[2][2], empty[2][2], scales[kScalePlaces], q_rows, q_full, s_full[kScoreTiles], p_full[kScoreTiles], pv_done[kScoreTiles], drained;
+  uint64_t full[2][2], empty[2][2], scales[kScalePlaces], q_rows, q_full, drained;
+  uint64_t s_full[kScoreTiles], p_full[kScoreTiles], pv_done[kScoreTiles];
   float m[kTileQ], sum[kTileQ], l[2][kTileQ], lm[2][kTileQ];
   uint32_t tmem;
   int failed;
@@ -741,7 +747,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) paged_tile_kernel(const Paged
     // have seen the phase before the one that it has waited for, whose parity then lets it through at once; the other
     // group's wait is sure, so the reads of O come after the barrier of both and a fence behind it.
     __syncwarp();
-    sh.l[half][row] = expired ? __int_as_float(0x7fc00000) : row_l;  // no number is taken for a result after an expired wait
+    sh.l[half][row] = expired ? __int_as_float(0x7fc00000) : row_l;  // an expired wait leaves no number in its rows
     sh.lm[half][row] = row_m;
     tc_before();
     asm volatile("bar.sync 1, 256;\n" ::: "memory");

@@ -9,14 +9,17 @@
 // shared memory); from there each works on whole (page, head) pairs alone: a
 // few warps a head, four rows of K and V a warp held in registers from the load
 // (issued before the norm's barrier) to the codes.  q's arithmetic is
-// nh_prefill_qk's; K's norm and rotation are in 64 bits, rounded to f32 once, so
+// nh_prefill_qk's, but for the order in which the 64-bit sum of squares is added
+// up (by heads over the CTAs); K's norm and rotation are in 64 bits, rounded to f32 once, so
 // that a value next to a code's border falls on the side where it belongs.
 //
 // What bounds it: one row a sequence, the chain of dependent loads and the
-// cluster's barrier (one sequence 9.3 us on the GPU, 64 sequences 15.2 us);
-// prompts, the instructions between the loads and that barrier (16 prompts of up
-// to 600 rows, 16 heads of 128: 118 us where the bytes take 50; q and K are read
-// a second time, out of L2, after the norm is known).
+// cluster's barrier (one sequence 6.6 us on the GPU, 64 sequences 7.7, each among
+// others in a graph); prompts (16 of up to 600 rows, 16 heads of 128: 95 us where
+// the bytes take 37), not HBM nor the issue slots, which are 36% busy with 47% of
+// the warps' places taken (counters): the loads before that barrier and what
+// follows it lie one after the other.  q and K are read a second time, out of L2,
+// after the norm is known.
 #include <cooperative_groups.h>
 #include <cuda_bf16.h>
 
@@ -453,8 +456,9 @@ constexpr int kReadThreads = 256;
 constexpr int kReadRows = 4;  // rows of a CTA, a quarter of its threads each
 constexpr int kReadAhead = 2;
 
-// CTA (c, s): rows c * kReadRows .. of sequence s, sixteen values a thread at a time.  Bound by its stores: 32,000 rows of
-// 16 heads of 128 as f32 take 145 us, 4.5 TB/s.
+// CTA (c, s): rows c * kReadRows .. of sequence s, sixteen values a thread at a time.  Bound by its stores, a thread's 64
+// (f32) or 32 bytes apart from its neighbour's: 32,000 rows of 16 heads of 128 take 148 us as f32 (4.4 TB/s), 76 as bf16
+// (5.2 TB/s).
 __global__ void __launch_bounds__(kReadThreads) paged_read_kernel(const ReadArgs p) {
   constexpr int kPart = kReadThreads / kReadRows;
   pdl_wait();
@@ -553,7 +557,7 @@ extern "C" int nh_paged_append(const NhPagedKv* kv, const NhPagedRows* rows, con
                                           p.rows.max_blocks);
   if (pages > 65535) return NH_E_ARG;
   // CTAs of a page: more heads each where the pages alone fill the machine (the sums and the barrier cost a CTA the same
-  // for any number of heads): the prompts above take 146 us with eight CTAs a page, 118 with four, 127 with two; one
+  // for any number of heads): the prompts above take 121 us with eight CTAs a page, 95 with four, 106 with two; one
   // page alone is quickest with eight.
   int ranks = std::min(kMaxRanks, p.kv.n_kv);
   if (ranks == kMaxRanks && pages * p.rows.n_seq > 200) ranks = 4;

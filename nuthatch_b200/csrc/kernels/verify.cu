@@ -11,8 +11,8 @@
 //
 // What bounds it: few sequences, the chain of dependent loads (offsets, ids,
 // probabilities, row) and the two searches (4 drafts of one sequence over 50,304
-// ids: 6.9 us, most of it the launch); many, the rows' bytes (64 sequences of up
-// to 5 drafts 11 us, 256 of up to 7 without draft rows 16.5 us: 3.1 TB/s).
+// ids: 7.0 us, most of it the launch); many, the rows' bytes (64 sequences of up
+// to 5 drafts with their rows 11.3 us, 256 of up to 7 without 16.6 us: 3.1 TB/s).
 #include <cooperative_groups.h>
 
 #include "common.cuh"
@@ -286,8 +286,9 @@ extern "C" int nh_verify_drafts(const NhVerifyDrafts* d, void* stream) {
       static_cast<int64_t>(d->n_drafts) + d->n_seq > INT32_MAX)
     return NH_E_ARG;
   if (d->n_drafts > 0 && (d->draft_ids == nullptr || d->u_accept == nullptr)) return NH_E_ARG;
-  // CTAs of a sequence: eight unless the sequences alone fill the machine twice.  (64 and 256 sequences: 11.3 and 26.7 us
-  // up to 300 CTAs, 16.4 and 32.7 up to 600, 16.6 and 43 up to 1,200, where each CTA's searches are the more work.)
+  // CTAs of a sequence: eight unless the sequences alone fill the machine twice.  (Up to 5 drafts with their rows of 64
+  // and of 256 sequences, up to 7 without of 256: 11.9, 26.7 and 17.1 us up to 300 CTAs; 17.6, 32.6 and 23.6 up to 600;
+  // 17.6, 42.3 and 36.4 up to 1,200, where the CTAs' searches are the more work.)
   int ranks = kMaxRanks;
   while (ranks > 1 && static_cast<int64_t>(d->n_seq) * ranks > 300) ranks /= 2;
   return launch_cluster(verify_drafts_kernel, dim3(ranks, d->n_seq), dim3(kVerifyThreads), ranks, 0,

@@ -508,7 +508,8 @@ int nh_paged_append(const NhPagedKv* kv, const NhPagedRows* rows, const float* q
  * calls give equal bits.  A row that sees no position gives zeros.  A bounded
  * wait inside the kernel that expires makes its rows NaN and records NH_E_TIMEOUT
  * in *err (where no other code stands there yet).  max_rows * n_head / n_head_kv
- * is below 2^31. */
+ * is below 2^31, and so are the call's blocks of 128 rows and heads, n_rows *
+ * n_head / 128 + n_seq * n_head_kv. */
 int nh_paged_attention(const NhPagedKv* kv, const NhPagedRows* rows, const float* qr, int n_head, float kq_scale,
                        int window, int n_sink, float* out, void* stream);
 

@@ -691,6 +691,7 @@ extern "C" int nh_paged_attention(const NhPagedKv* kv, const NhPagedRows* rows, 
   p.few = INT32_MAX;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   if (static_cast<int64_t>(p.rows.max_rows) * p.group <= kFewQueries) return launch_paged_split(p, st);
+  if (paged_tiles(p) * p.kv.n_kv > INT32_MAX) return NH_E_ARG;
   if (p.rows.n_seq == 1) {
     p.few = 0;
     return launch_paged_tiles(p, st);

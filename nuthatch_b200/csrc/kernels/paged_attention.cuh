@@ -90,4 +90,11 @@ __device__ __forceinline__ float2 add2(float2 a, float2 b) {
 int launch_paged_split(const PagedAttnArgs& p, cudaStream_t s);
 int launch_paged_tiles(const PagedAttnArgs& p, cudaStream_t s);
 
+// Tiles of a call at most: no more than whole ones of all rows and a part of one for each sequence, nor than every
+// sequence's most.
+inline int64_t paged_tiles(const PagedAttnArgs& p) {
+  const int64_t most = static_cast<int64_t>(p.rows.max_rows) * p.group;
+  return std::min(static_cast<int64_t>(p.rows.n_rows) * p.group / 128 + p.rows.n_seq, p.rows.n_seq * ((most + 127) / 128));
+}
+
 }  // namespace nh

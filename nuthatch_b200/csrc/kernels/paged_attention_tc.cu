@@ -822,7 +822,6 @@ int launch_tiles(const PagedAttnArgs& p, int64_t tiles, cudaStream_t s) {
   const int64_t items = tiles * p.kv.n_kv, steps = static_cast<int64_t>(p.rows.max_blocks) * p.kv.page / kTileK;
   int ranks = 1;
   while (ranks < 8 && items * ranks * 2 <= device_sm_count() && steps >= 4 * ranks) ranks *= 2;
-  if (items * ranks > INT32_MAX) return NH_E_ARG;
   return launch_cluster(paged_tile_kernel<HD>, dim3(static_cast<unsigned>(items * ranks)), dim3(kTileThreads), ranks, smem,
                         s, p);
 }
@@ -830,10 +829,8 @@ int launch_tiles(const PagedAttnArgs& p, int64_t tiles, cudaStream_t s) {
 }  // namespace
 
 int launch_paged_tiles(const PagedAttnArgs& p, cudaStream_t s) {
-  const int64_t most = static_cast<int64_t>(p.rows.max_rows) * p.group;
-  // No more tiles than whole ones of all rows and a part of one for each sequence, nor than every sequence's most.
-  const int64_t tiles = std::min(static_cast<int64_t>(p.rows.n_rows) * p.group / kTileQ + p.rows.n_seq,
-                                 p.rows.n_seq * ((most + kTileQ - 1) / kTileQ));
+  static_assert(kTileQ == 128, "paged_tiles");
+  const int64_t tiles = paged_tiles(p);
   switch (p.kv.hd) {
     case 32:
       return launch_tiles<32>(p, tiles, s);

@@ -465,8 +465,8 @@ typedef struct NhPagedKv {
  * such a sequence's rows are left as they were, such a page's positions are
  * neither written nor seen.  A page of which no row of the call sees or writes
  * a position (behind the window, past the last row) may have any entry.  Rows
- * at and after row_off[n_seq] are left as they were.  A page that is written belongs to one sequence of the call; pages
- * that are only read may be shared. */
+ * at and after row_off[n_seq] are left as they were.  A page that is written
+ * belongs to one sequence of the call; pages that are only read may be shared. */
 typedef struct NhPagedRows {
   int32_t n_seq;      /* 1 .. 65535 */
   int32_t max_rows;

@@ -4,9 +4,9 @@
 // A CTA takes up to 2, 4, 8 or 16 queries of one (sequence, KV head) and a
 // contiguous part of the positions; a cluster's CTAs split the positions and
 // join their (maximum, sum, weighted values) through distributed shared memory
-// in rank order.  A warp takes units of 16 positions, always inside one page, through a
-// ring of stages of its own in shared memory (cp.async, no barrier between
-// warps), and reads them in the operand layout of mma.m16n8k16: both the
+// in rank order.  A warp takes units of 16 positions, always inside one page,
+// through a ring of stages of its own in shared memory (cp.async, no barrier
+// between warps), and reads them in the operand layout of mma.m16n8k16: both the
 // dimensions of K and those of V may be permuted freely, so each lane reads
 // whole 16-byte pieces.
 //   2 queries: the scores by integer products (m16n8k32), K's codes as they

@@ -10,8 +10,8 @@
 // few warps a head, four rows of K and V a warp held in registers from the load
 // (issued before the norm's barrier) to the codes.  q's arithmetic is
 // nh_prefill_qk's, but for the order in which the 64-bit sum of squares is added
-// up (by heads over the CTAs); K's norm and rotation are in 64 bits, rounded to f32 once, so
-// that a value next to a code's border falls on the side where it belongs.
+// up (by heads over the CTAs); K's norm and rotation are in 64 bits, rounded to
+// f32 once, so that a value next to a code's border falls on the side where it belongs.
 //
 // What bounds it: one row a sequence, the chain of dependent loads and the
 // cluster's barrier (one sequence 6.6 us on the GPU, 64 sequences 7.7, each among
